@@ -396,6 +396,12 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
 #define WASTE_CUDA_DERR_PEER_WAIT  8u   /* expert parallel: a peer's token or partial-sum
                                            flag did not arrive (a rank that did not make
                                            the call); the layer's outputs are not valid */
+#define WASTE_CUDA_DERR_BAD_BLOCK 16u  /* a paged-cache call met a block id, a cache row or a
+                                           length outside the cache or its table; that request's
+                                           results are not valid, nothing outside was touched */
+#define WASTE_CUDA_DERR_BAD_TREE  32u  /* kv_plan: a parent that is no earlier node (taken as a
+                                           root), a tree of more than 32 * mask_words nodes (not
+                                           served), or more new tokens than T (left out) */
 unsigned waste_cuda_device_errors(void);
 
 /* ---- single VQ3R kernels ---------------------------------------------------
@@ -629,6 +635,164 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
                                     const void *const *sel, const uint16_t *const *scale,
                                     const float *const *x, float *const *y, int M, int N,
                                     int cb_base, int stages, int copies, void *stream);
+
+/* ---- the serving step over a paged latent cache ---------------------------
+ * What a batch of requests with one or several new tokens each goes
+ * through around the layers, where mla_layer decodes one token of one
+ * request over a contiguous fp32 cache: kv_plan makes the step's maps on
+ * the device from the requests' lengths, mla_rows writes the new latents
+ * into the paged cache, mla_tree_attn attends over it, and logits_adjust
+ * prepares the rows of logits for sampling. No counterpart in the reference,
+ * which runs one sequence.
+ *
+ * All four take a descriptor of sizes and device pointers that the call
+ * only reads (it can be kept and handed over at every step), are ordered
+ * on `stream`, allocate nothing, copy nothing and hold no state between
+ * calls, so they can be captured into a CUDA graph and calls on different
+ * streams are independent (mla_tree_attn: each with its own workspace).
+ * stream NULL is the library's own stream; cudaStreamLegacy names the
+ * default stream. The calling thread's current device must be the one the
+ * library is bound to. Lengths, ids and tables are read on the device
+ * only; a value out of range there never moves an access outside the
+ * caller's buffers: it raises a bit of waste_cuda_device_errors.
+ *
+ * A new token t of request r is row t of the step's arrays, with
+ * q_indptr[r] <= t < q_indptr[r+1]. Its latent lies in the cache at the
+ * request's position ctx + (t - q_indptr[r]), whatever its depth in a
+ * tree; a position p lies in block block_table[r][p / page] at row
+ * p % page of it, i.e. in cache row block * page + p % page. */
+#define WASTE_CUDA_F32  0
+#define WASTE_CUDA_F16  1
+#define WASTE_CUDA_BF16 2
+
+/* Block tables, cache rows, positions and ancestor masks from lengths.
+ * Request r holds n_blocks[r] blocks (the first n_blocks[r] entries of its
+ * table row) and ctx_len[r] rows, and gets q_len[r] >= 0 new tokens. It
+ * needs ceil((ctx + q) / page) blocks; what it lacks is taken from
+ * free_blocks[*free_head ..), requests in ascending order. A request whose
+ * share does not fit what is left, behind all before it, is not served
+ * (and takes nothing): kv_len 0, slots -1. Neither is one whose blocks
+ * exceed max_blocks or whose lengths are negative (BAD_BLOCK).
+ *   parent     NULL: the new tokens are a chain (a prompt's chunk, or one
+ *              token). Else [T]: the parent of each node as an index among
+ *              its request's new tokens, smaller than its own, or -1 for a
+ *              child of the last cached token.
+ *   n_blocks_out, free_head_out   the counts after the step; each may be
+ *              its input's array
+ *   block_table   the new entries are written, the others left as they are
+ *   q_indptr [B+1], kv_len [B] (rows with the new ones), pos [T] (rotary
+ *   position: ctx + depth), slot [T] (cache row), mask [T][mask_words]
+ *   (bit j: node j is an ancestor or the node itself; NULL allowed with a
+ *   chain), short_blocks [1] (blocks that lacked, 0 if none).
+ * T: rows of the per-token arrays; rows behind the last request's are left
+ * as they are. B <= 4096; q <= 32 * mask_words where a mask is written. */
+typedef struct {
+    int B, T, page, max_blocks, n_free, mask_words;
+    const int *ctx_len, *q_len, *parent, *free_blocks, *free_head, *n_blocks;
+    int *block_table;                            /* [B][max_blocks] */
+    int *free_head_out, *n_blocks_out;
+    int *q_indptr, *kv_len, *pos;
+    int64_t *slot;
+    uint32_t *mask;
+    int *short_blocks;
+} waste_cuda_kv_plan_desc;
+int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream);
+
+/* The new tokens' latents into the cache: row t of x (x_stride elements
+ * apart, F32, F16 or BF16: the output of kv_a_proj_with_mqa) is normalised
+ * over its first kl values (rmsnorm with norm_w, as mla_layer does), its
+ * rope values rotated in pairs (2j, 2j+1) by pos[t] * inv_freq[j]
+ * (inv_freq NULL: NoPE), and kl + rope values are rounded to `dtype` into
+ * cache row slot[t] (row_stride elements apart; n_rows rows). A negative
+ * slot skips its token; slots of one call are distinct. Sums, angles and
+ * the rotation in at least 32 bits (the angle in 64). kl 1..4096, rope even,
+ * 0..512. */
+typedef struct {
+    int T, kl, rope, x_dtype, dtype;
+    size_t x_stride;
+    const void *x;
+    const float *norm_w, *inv_freq;              /* [kl], [rope / 2]      */
+    const int *pos;
+    const int64_t *slot;
+    float eps;
+    void *cache;
+    size_t row_stride;
+    int64_t n_rows;
+} waste_cuda_mla_rows_desc;
+int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
+
+/* Absorbed MLA attention of every new token over its request's cache rows:
+ * for token t and head h, s_p = scale * q[t][h] . c_p over the kl + rope
+ * values of the rows p it sees, o[t][h] = softmax(s) . c[:kl], and
+ * lse[t][h] = log(sum exp(s)) (NULL: not written). Seen are the cached rows
+ * p < kv_len[r] - q_len[r], and among the request's new ones row j if bit j
+ * of mask[t] is set; with mask NULL, the rows up to the token's own
+ * (a chain). A token that sees nothing (as in a request with kv_len <
+ * q_len, e.g. one that kv_plan did not serve) gets o = 0 and lse =
+ * -infinity. What a row holds (a NaN, an infinity) reaches the tokens that
+ * see it and no others.
+ * q and o are of the cache's type `dtype`; scores, the softmax and sums in
+ * 32 bits; with 16-bit types the weights are rounded to the type for the
+ * product with the rows (their sum and lse are of the unrounded ones). o is
+ * [T][heads][kl] and q [T][heads][kl + rope] at the given strides in
+ * elements; rows behind q_indptr[B] are left as they are. kl 1..512, rope
+ * 0..128, page >= 1, mask_words * 32 >= the most new tokens of a request.
+ * n_blocks: blocks in the cache. ws: waste_cuda_mla_tree_ws_bytes(heads,
+ * kl) bytes on the device, 256-byte aligned, not shared by calls that may
+ * overlap (another stream, another captured graph); nothing in it has to
+ * be set, or survives the call. Results do not depend on what runs beside
+ * the call: sums are in a fixed order. */
+typedef struct {
+    int B, T, heads, kl, rope, dtype, page, max_blocks, mask_words;
+    int64_t n_blocks;
+    size_t row_stride, q_token_stride, q_head_stride, o_token_stride, o_head_stride;
+    const void *q, *cache;
+    const int *block_table, *kv_len, *q_indptr;
+    const uint32_t *mask;
+    float scale;
+    void *o;
+    float *lse;
+    void *ws;
+    size_t ws_bytes;
+} waste_cuda_mla_tree_desc;
+size_t waste_cuda_mla_tree_ws_bytes(int heads, int kl);
+int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream);
+
+/* Rows of logits made ready for sampling. Request r has rows
+ * q_indptr[r] <= t < q_indptr[r+1] (q_indptr NULL: row r, R = B). In this
+ * order, for each id v of a row (x in 32 bits, rounded to `dtype` at the
+ * end):
+ *   if v was seen      x = x > 0 ? x / rep[r] : x * rep[r]
+ *   x -= freq[r] * n(v) + pres[r] * (n(v) > 0)    n: times v was produced
+ *   x += bias of v (where the request's list names it; of equal ids the
+ *        last holds)
+ *   x = -infinity      where the row's grammar mask has no bit v
+ * Seen are the request's tokens hist[r][0 .. hist_len[r]); produced are
+ * those from prompt_len[r] on. draft [R] (NULL: none): the row's node's
+ * drafted token; the tokens of the node and its ancestors (bits of
+ * tree[t], tree_words words; NULL: the rows up to its own) count as seen
+ * and produced for that row. bias_id / bias_val: request r's entries are
+ * bias_indptr[r] .. bias_indptr[r+1] (NULL: none). allow
+ * [n_allow][allow_words] bits (NULL: none): row t is under mask
+ * allow_row[t], or under none if that is negative; allow_row NULL: mask t.
+ * rep, freq, pres, hist NULL: 1, 0, 0, empty. Ids outside 0..V-1 are
+ * ignored. ld, ld_out: elements between rows; out may be logits with the
+ * same ld. Rows behind q_indptr[B] are left as they are. */
+typedef struct {
+    int B, R, V, dtype, tree_words, allow_words, n_allow;
+    size_t hist_stride, ld, ld_out;
+    const void *logits;
+    void *out;
+    const int *q_indptr, *hist, *hist_len, *prompt_len;
+    const float *rep, *freq, *pres;
+    const int *draft;
+    const uint32_t *tree;
+    const int *bias_indptr, *bias_id;
+    const float *bias_val;
+    const uint32_t *allow;
+    const int *allow_row;
+} waste_cuda_logits_desc;
+int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream);
 
 /* Kernels this library launched since load (a running count, for
  * benchmarks that report how many of their launches were this library's). */

@@ -42,6 +42,8 @@ EXPORTS = (
     "waste_cuda_kda_step_dev", "waste_cuda_short_conv_dev", "waste_cuda_rmsnorm_gated_dev",
     "waste_cuda_vq_encode", "waste_cuda_vq_encode_dev", "waste_cuda_vq_lloyd",
     "waste_cuda_vq_lloyd_dev", "waste_cuda_kda_layer", "waste_cuda_mla_layer",
+    "waste_cuda_kv_plan_dev", "waste_cuda_mla_rows_dev", "waste_cuda_mla_tree_ws_bytes",
+    "waste_cuda_mla_tree_attn_dev", "waste_cuda_logits_adjust_dev",
 )
 
 PHASES = ("router", "act", "gateup", "down", "combine", "matvec", "matvec_reduce", "ep_publish",
@@ -49,6 +51,8 @@ PHASES = ("router", "act", "gateup", "down", "combine", "matvec", "matvec_reduce
 
 OK, E_ARG, E_DEVICE, E_RECORD, E_NOBANK, E_NOMEM, E_NODEV = 0, -1, -2, -3, -4, -5, -6
 DERR_ROUTE_WAIT, DERR_TMA_WAIT, DERR_BAD_EXPERT, DERR_PEER_WAIT = 1, 2, 4, 8
+DERR_BAD_BLOCK, DERR_BAD_TREE = 16, 32
+F32, F16, BF16 = 0, 1, 2
 
 
 class WasteCudaError(RuntimeError):
@@ -84,6 +88,48 @@ class VqSlots(C.Structure):
                 ("rmsnorm_gated_heads", C.c_void_p), ("moe_trunk_load", C.c_void_p),
                 ("moe_activation", C.c_void_p), ("moe_layer", C.c_void_p),
                 ("kda_layer", C.c_void_p), ("mla_layer", C.c_void_p)]
+
+
+class KvPlan(C.Structure):
+    """waste_cuda_kv_plan_desc: sizes and device pointers of kv_plan_dev."""
+    _fields_ = ([(n, C.c_int) for n in ("B", "T", "page", "max_blocks", "n_free", "mask_words")] +
+                [(n, C.c_void_p) for n in
+                 ("ctx_len", "q_len", "parent", "free_blocks", "free_head", "n_blocks",
+                  "block_table", "free_head_out", "n_blocks_out", "q_indptr", "kv_len", "pos",
+                  "slot", "mask", "short_blocks")])
+
+
+class MlaRows(C.Structure):
+    """waste_cuda_mla_rows_desc: sizes and device pointers of mla_rows_dev."""
+    _fields_ = ([(n, C.c_int) for n in ("T", "kl", "rope", "x_dtype", "dtype")] +
+                [("x_stride", C.c_size_t)] +
+                [(n, C.c_void_p) for n in ("x", "norm_w", "inv_freq", "pos", "slot")] +
+                [("eps", C.c_float), ("cache", C.c_void_p), ("row_stride", C.c_size_t),
+                 ("n_rows", C.c_int64)])
+
+
+class MlaTree(C.Structure):
+    """waste_cuda_mla_tree_desc: sizes and device pointers of mla_tree_attn_dev."""
+    _fields_ = ([(n, C.c_int) for n in ("B", "T", "heads", "kl", "rope", "dtype", "page",
+                                        "max_blocks", "mask_words")] +
+                [("n_blocks", C.c_int64)] +
+                [(n, C.c_size_t) for n in ("row_stride", "q_token_stride", "q_head_stride",
+                                           "o_token_stride", "o_head_stride")] +
+                [(n, C.c_void_p) for n in ("q", "cache", "block_table", "kv_len", "q_indptr",
+                                           "mask")] +
+                [("scale", C.c_float), ("o", C.c_void_p), ("lse", C.c_void_p), ("ws", C.c_void_p),
+                 ("ws_bytes", C.c_size_t)])
+
+
+class LogitsAdjust(C.Structure):
+    """waste_cuda_logits_desc: sizes and device pointers of logits_adjust_dev."""
+    _fields_ = ([(n, C.c_int) for n in ("B", "R", "V", "dtype", "tree_words", "allow_words",
+                                        "n_allow")] +
+                [(n, C.c_size_t) for n in ("hist_stride", "ld", "ld_out")] +
+                [(n, C.c_void_p) for n in
+                 ("logits", "out", "q_indptr", "hist", "hist_len", "prompt_len", "rep", "freq",
+                  "pres", "draft", "tree", "bias_indptr", "bias_id", "bias_val", "allow",
+                  "allow_row")])
 
 
 _lib = None
@@ -179,6 +225,11 @@ def load_library() -> C.CDLL:
         "waste_cuda_vq_lloyd_dev": (C.c_int, [P, C.c_int, P, C.c_int, C.c_int, P, P]),
         "waste_cuda_kda_layer": (C.c_int, [P, P, P]),
         "waste_cuda_mla_layer": (C.c_int, [P, C.c_int, P, P]),
+        "waste_cuda_kv_plan_dev": (C.c_int, [C.POINTER(KvPlan), P]),
+        "waste_cuda_mla_rows_dev": (C.c_int, [C.POINTER(MlaRows), P]),
+        "waste_cuda_mla_tree_ws_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+        "waste_cuda_mla_tree_attn_dev": (C.c_int, [C.POINTER(MlaTree), P]),
+        "waste_cuda_logits_adjust_dev": (C.c_int, [C.POINTER(LogitsAdjust), P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)
@@ -633,3 +684,34 @@ def vq_lloyd_dev(d_X, n, d_C, entries, dim, d_live, stream: int = 0):
     v = lambda p: C.c_void_p(int(p)) if p else None
     _check(load_library().waste_cuda_vq_lloyd_dev(v(d_X), n, v(d_C), entries, dim, v(d_live),
                                                   v(stream)))
+
+
+# ---- the serving step over a paged latent cache ----------------------------------
+
+def kv_plan_dev(d: KvPlan, stream: int = 0):
+    """Block tables, cache rows, positions and ancestor masks of a step's new
+    tokens from the requests' lengths (see waste_cuda_kv_plan_dev)."""
+    _check(load_library().waste_cuda_kv_plan_dev(d, stream or None))
+
+
+def mla_rows_dev(d: MlaRows, stream: int = 0):
+    """The new tokens' latents normalised, rotated and stored at their cache
+    rows (see waste_cuda_mla_rows_dev)."""
+    _check(load_library().waste_cuda_mla_rows_dev(d, stream or None))
+
+
+def mla_tree_ws_bytes(heads: int, kl: int) -> int:
+    """Bytes of workspace mla_tree_attn_dev needs (0 before init)."""
+    return int(load_library().waste_cuda_mla_tree_ws_bytes(heads, kl))
+
+
+def mla_tree_attn_dev(d: MlaTree, stream: int = 0):
+    """Absorbed MLA attention of the new tokens, a chain or a tree of drafts
+    each, over the paged cache (see waste_cuda_mla_tree_attn_dev)."""
+    _check(load_library().waste_cuda_mla_tree_attn_dev(d, stream or None))
+
+
+def logits_adjust_dev(d: LogitsAdjust, stream: int = 0):
+    """Penalties for repeated tokens, biases and grammar masks on rows of
+    logits (see waste_cuda_logits_adjust_dev)."""
+    _check(load_library().waste_cuda_logits_adjust_dev(d, stream or None))

@@ -24,7 +24,7 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 CU_SOURCES = ["vq3r_kernels.cu", "prefill_tc.cu", "trunk_mvq.cu", "matvec_sel.cu", "vq4p.cu", "kda.cu",
-              "vq_encode.cu", "mla.cu"]
+              "vq_encode.cu", "mla.cu", "serve_step.cu", "mla_tree.cu"]
 C_SOURCES = ["waste_cuda.c"]
 HEADERS = ["vq3r_common.cuh", "wc_launch.h", "pdl.cuh"]
 

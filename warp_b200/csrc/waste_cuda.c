@@ -119,6 +119,9 @@ static struct {
     /* the encoder's buffers (host-pointer forms) and the Lloyd scratch */
     void *d_enc;
     size_t enc_bytes;
+    /* the serving step: its sticky error word and the SM count */
+    unsigned int *d_serr;
+    int sms;
 } S;
 
 /* Bumped by every call that allocates, frees or reloads what a cached
@@ -262,7 +265,12 @@ static unsigned read_device_errors(int clear)
 unsigned waste_cuda_device_errors(void)
 {
     pthread_mutex_lock(&g_mu);
-    const unsigned v = S.inited ? read_device_errors(1) : 0;
+    unsigned v = S.inited ? read_device_errors(1) : 0;
+    if (S.inited && v != ~0u) {
+        unsigned int w = 0;
+        if (cudaMemcpy(&w, S.d_serr, sizeof w, cudaMemcpyDeviceToHost) != cudaSuccess) v = ~0u;
+        else if (w) { memset_now(S.d_serr, 0, sizeof w); v |= w; }
+    }
     pthread_mutex_unlock(&g_mu);
     return v;
 }
@@ -376,6 +384,9 @@ static int init_locked(int device)
     /* the allocation-free matvec's array and kernels, on the device now */
     CK((cudaError_t)wc_noalloc_setup(&g_noalloc_part), "fixed scratch set-up");
     if (!g_noalloc_part) return fail(WASTE_CUDA_E_DEVICE, "fixed scratch address: NULL");
+    CK(cudaMalloc((void **)&S.d_serr, 256), "serving error word");
+    CK(memset_now(S.d_serr, 0, 256), "serving error word");
+    S.sms = p.multiProcessorCount;
     CK(cudaMalloc((void **)&S.d_idx, (size_t)WC_CHUNK_MAX * WC_MAX_TOPK * sizeof(int)), "idx");
     CK(cudaMalloc((void **)&S.d_w, (size_t)WC_CHUNK_MAX * WC_MAX_TOPK * sizeof(float)), "w");
     CK(cudaMallocHost((void **)&S.h_idx, (size_t)WC_CHUNK_MAX * WC_MAX_TOPK * sizeof(int)), "h_idx");
@@ -438,6 +449,7 @@ void waste_cuda_shutdown(void)
         cudaFree(S.d_res); cudaFreeHost(S.h_res);
         cudaFree(S.d_p6);
         cudaFree(S.d_enc);
+        cudaFree(S.d_serr);
         mirrors_free();
         states_free();
         for (int b = 0; b < 2; b++) {
@@ -3281,6 +3293,131 @@ int waste_cuda_vq_dequant(float *W, const uint8_t *idx, const uint16_t *scale, i
                                       S.stream), "dequant");
     CK(cudaMemcpyAsync(W, d_W, wb, cudaMemcpyDeviceToHost, S.stream), "W D2H");
     CK(cudaStreamSynchronize(S.stream), "dequant");
+out:
+    pthread_mutex_unlock(&g_mu);
+    return rc;
+}
+
+/* ---- the serving step over a paged latent cache -------------------------- */
+
+static size_t dtype_size(int dtype)
+{
+    return dtype == WASTE_CUDA_F32 ? 4 : dtype == WASTE_CUDA_F16 || dtype == WASTE_CUDA_BF16 ? 2 : 0;
+}
+
+static int misaligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
+
+/* The caller holds g_mu: the library is bound and its device is current. */
+static int serve_ready(const char *what)
+{
+    int dev = -1;
+    if (!S.inited) return fail(WASTE_CUDA_E_NODEV, "%s before waste_cuda_init", what);
+    if (cudaGetDevice(&dev) != cudaSuccess || dev != S.device)
+        return fail(WASTE_CUDA_E_ARG, "%s: the current device is %d, the library's %d", what, dev,
+                    S.device);
+    return 0;
+}
+
+int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream)
+{
+    int rc = 0;
+    if (!d || d->B < 1 || d->B > 4096 || d->T < 0 || d->page < 1 || d->max_blocks < 1 ||
+        (int64_t)d->page * d->max_blocks > INT32_MAX || d->n_free < 0 ||
+        (d->n_free > 0 && !d->free_blocks) || !d->ctx_len || !d->q_len || !d->free_head ||
+        !d->n_blocks || !d->block_table || !d->free_head_out || !d->n_blocks_out || !d->q_indptr ||
+        !d->kv_len || (d->T > 0 && (!d->pos || !d->slot)) || !d->short_blocks)
+        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: bad sizes or a missing array (B 1..4096)");
+    if ((d->mask && d->mask_words < 1) || (d->parent && !d->mask))
+        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: a tree needs a mask of mask_words >= 1");
+    if (d->kv_len == d->ctx_len || d->kv_len == d->q_len || d->q_indptr == d->ctx_len ||
+        d->q_indptr == d->q_len || d->n_blocks_out == d->ctx_len || d->n_blocks_out == d->q_len ||
+        d->n_blocks_out == d->kv_len || misaligned(d->slot, 8))
+        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: only the counts may be updated in place");
+    pthread_mutex_lock(&g_mu);
+    if ((rc = serve_ready("kv_plan_dev"))) goto out;
+    CK((cudaError_t)wc_kv_plan_launch(d, S.d_serr, stream ? stream : (void *)S.stream), "kv_plan");
+out:
+    pthread_mutex_unlock(&g_mu);
+    return rc;
+}
+
+int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream)
+{
+    int rc = 0;
+    if (!d || d->T < 0 || d->kl < 1 || d->kl > 4096 || d->rope < 0 || d->rope > 512 ||
+        (d->rope & 1) || !dtype_size(d->dtype) || !dtype_size(d->x_dtype) ||
+        d->x_stride < (size_t)(d->kl + d->rope) || d->row_stride < (size_t)(d->kl + d->rope) ||
+        d->n_rows < 0 || !(d->eps >= 0.0f))
+        return fail(WASTE_CUDA_E_ARG, "mla_rows_dev: bad sizes or types (kl 1..4096, rope even, 0..512)");
+    if (d->T == 0) return 0;
+    if (!d->x || !d->norm_w || !d->slot || !d->cache || (d->inv_freq && !d->pos) ||
+        misaligned(d->x, dtype_size(d->x_dtype)) || misaligned(d->cache, dtype_size(d->dtype)))
+        return fail(WASTE_CUDA_E_ARG, "mla_rows_dev: a missing or misaligned array");
+    pthread_mutex_lock(&g_mu);
+    if ((rc = serve_ready("mla_rows_dev"))) goto out;
+    CK((cudaError_t)wc_mla_rows_launch(d, S.d_serr, stream ? stream : (void *)S.stream), "mla_rows");
+out:
+    pthread_mutex_unlock(&g_mu);
+    return rc;
+}
+
+size_t waste_cuda_mla_tree_ws_bytes(int heads, int kl)
+{
+    if (heads < 1 || kl < 1 || kl > 512) return 0;
+    pthread_mutex_lock(&g_mu);
+    const size_t n = S.inited ? wc_mla_tree_ws_bytes(kl, S.sms) : 0;
+    pthread_mutex_unlock(&g_mu);
+    return n;
+}
+
+int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream)
+{
+    int rc = 0;
+    if (!d || d->B < 0 || d->T < 0 || d->heads < 1 || d->kl < 1 || d->kl > 512 || d->rope < 0 ||
+        d->rope > 128 || !dtype_size(d->dtype) || d->page < 1 || d->max_blocks < 1 ||
+        (int64_t)d->page * d->max_blocks > INT32_MAX || d->n_blocks < 0 ||
+        (int64_t)d->T * d->heads > INT32_MAX || d->row_stride < (size_t)(d->kl + d->rope) ||
+        d->q_head_stride < (size_t)(d->kl + d->rope) || d->q_token_stride < (size_t)(d->kl + d->rope) ||
+        d->o_head_stride < (size_t)d->kl || d->o_token_stride < (size_t)d->kl ||
+        !(d->scale - d->scale == 0.0f))
+        return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: bad sizes, types or strides (kl 1..512, rope 0..128)");
+    if (d->B == 0 || d->T == 0) return 0;
+    const size_t z = dtype_size(d->dtype);
+    if (!d->q || !d->cache || !d->block_table || !d->kv_len || !d->q_indptr || !d->o || !d->ws ||
+        (d->mask && d->mask_words < 1) || misaligned(d->q, z) || misaligned(d->cache, z) ||
+        misaligned(d->o, z) || misaligned(d->ws, 256))
+        return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
+    pthread_mutex_lock(&g_mu);
+    if ((rc = serve_ready("mla_tree_attn_dev"))) goto out;
+    if (d->ws_bytes < wc_mla_tree_ws_bytes(d->kl, S.sms)) {
+        rc = fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: workspace of %zu bytes, %zu needed", d->ws_bytes,
+                  wc_mla_tree_ws_bytes(d->kl, S.sms));
+        goto out;
+    }
+    CK((cudaError_t)wc_mla_tree_launch(d, S.d_serr, S.sms, stream ? stream : (void *)S.stream),
+       "mla_tree_attn");
+out:
+    pthread_mutex_unlock(&g_mu);
+    return rc;
+}
+
+int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream)
+{
+    int rc = 0;
+    if (!d || d->B < 0 || d->B > 65535 || d->R < 0 || d->V < 1 || d->V > INT32_MAX - 8192 ||
+        !dtype_size(d->dtype) || d->ld < (size_t)d->V || d->ld_out < (size_t)d->V ||
+        (!d->q_indptr && d->R != d->B))
+        return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: bad sizes, type or strides (B up to 65535)");
+    if (d->B == 0 || d->R == 0) return 0;
+    if (!d->logits || !d->out || (d->out == d->logits && d->ld != d->ld_out) ||
+        (d->hist && !d->hist_len) || (d->tree && (!d->draft || d->tree_words < 1)) ||
+        (d->bias_indptr && (!d->bias_id || !d->bias_val)) ||
+        (d->allow && ((int64_t)d->allow_words * 32 < d->V || d->n_allow < 0)) ||
+        misaligned(d->logits, dtype_size(d->dtype)) || misaligned(d->out, dtype_size(d->dtype)))
+        return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: a missing, short or misaligned array");
+    pthread_mutex_lock(&g_mu);
+    if ((rc = serve_ready("logits_adjust_dev"))) goto out;
+    CK((cudaError_t)wc_logits_launch(d, stream ? stream : (void *)S.stream), "logits_adjust");
 out:
     pthread_mutex_unlock(&g_mu);
     return rc;

@@ -6,6 +6,8 @@
 #ifndef WC_LAUNCH_H
 #define WC_LAUNCH_H
 
+#include "waste_cuda.h"
+
 #include <cuda.h>
 #include <stddef.h>
 #include <stdint.h>
@@ -354,6 +356,17 @@ int wc_mla_gate_launch(float *o, const float *g, int n, void *stream, int pdl);
 /* With pdl set, the head and the gate launch programmatically behind the
  * kernel before them: the head stages its kv_b_proj rows (constants) while
  * the prep runs. */
+
+/* The serving step over a paged latent cache (serve_step.cu, mla_tree.cu);
+ * the descriptors are the public ones of waste_cuda.h, checked by the
+ * caller. err: the sticky error word. sms: the device's SM count, which
+ * sizes the attention's grid and workspace. */
+int    wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, void *stream);
+int    wc_mla_rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, void *stream);
+size_t wc_mla_tree_ws_bytes(int kl, int sms);
+int    wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, unsigned int *err, int sms,
+                          void *stream);
+int    wc_logits_launch(const waste_cuda_logits_desc *d, void *stream);
 
 /* Phase timers (see waste_cuda_profile in include/waste_cuda.h). */
 enum { WC_PH_ROUTER, WC_PH_ACT, WC_PH_GATEUP, WC_PH_DOWN, WC_PH_COMBINE,
