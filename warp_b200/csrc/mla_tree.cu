@@ -25,6 +25,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <type_traits>
 
 using namespace wc;
 
@@ -409,6 +410,527 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
     }
 }
 
+/* ---- 16-bit caches on the tensor cores ---------------------------------------
+ * Transposed: the cache rows are the M side of both products, so 32 rows of
+ * queries (one token of 32 heads) fill an N of 32 and nothing is padded to
+ * 128:
+ *   S^T [128 keys x N]   = C [128 x (kl+rope)] . Q^T     A K-major
+ *   O^T [kl x N]        += C^T [kl x 128] . P^T          A M-major, same bytes
+ * One copy of the tile in shared memory serves both. N is 32 where a
+ * request's rows fit that, else 64: the cache is read once per 32 or 64 rows
+ * (the second by 64: one token of 64 heads, or two of 32).
+ *
+ * Shared memory (1 CTA an SM): a ring of 32 KB pairs (128 keys x 2 swizzled
+ * 64-column chunks) that TMA fills page by page, 5 pairs at N = 32 and 4 at
+ * N = 64; the rope chunk; the query tile; P. A tile's pairs are held from
+ * its first product to its last, which frees them one by one, so the next
+ * tile's loads run under the second product. At N = 64 P lies where the rope
+ * chunk was, which is read by then.
+ *
+ * Roles: warp 0 loads, one lane a box; a lane of warp 1 issues the products;
+ * warps 2..9 do the softmax, a thread a key (TMEM lane) and half of the
+ * columns: the column maxima by redux over the lanes and shared memory over
+ * the 4 warps, the weights rounded and stored as P. The running maximum is
+ * followed only when it grew by 2^kLazy or more (weights up to 2^kLazy are
+ * exact powers away, the sums are 32 bits wide), so O in TMEM is rescaled a
+ * few times at the start of a long row and hardly after.
+ *
+ * Every wait is bounded: one that runs out raises WC_ERR_TMA_WAIT and
+ * `dead`, upon which the roles run out their loops without waiting, issue
+ * nothing more, and drain what is in flight. */
+constexpr int kTcThreads = 320;
+constexpr int kTcKeys = 128;
+constexpr int kPairBytes = 2 * kTcKeys * 128;
+constexpr float kLazy = 6.0f;
+constexpr int kMaxPairs = 5;
+
+template <int N> struct TcCfg {
+    static constexpr int pairs = N == 64 ? 4 : 5;
+    static constexpr int NC = N / 2;                          /* columns a thread   */
+    static constexpr int p_row = N * 2;                       /* bytes of a P row    */
+    static constexpr int off_rope = pairs * kPairBytes;
+    static constexpr int off_p = N == 64 ? off_rope : off_rope + kTcKeys * 128;
+    static constexpr int off_q = N == 64 ? off_rope + kTcKeys * 128 : off_p + kTcKeys * p_row;
+    static constexpr int off_ctl = off_q + 9 * N * 128;
+};
+
+struct TcCtl {
+    uint64_t pair_full[kMaxPairs], pair_empty[kMaxPairs];
+    uint64_t rope_full, rope_empty, q_full, s_full, p_ready, o_done, drain;
+    uint32_t tmem;
+    volatile int dead;
+    long long red[66];
+    float mx[2][2][4][32];           /* [parity][half][quadrant][column] maxima     */
+    float col[8][32];                /* a warp's broadcast of one value a column     */
+    unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
+};
+
+__device__ __forceinline__ bool tc_wait(TcCtl &c, uint64_t *bar, uint32_t parity, unsigned int *err)
+{
+    for (int i = 0; i < kMbarLimit; i++) {
+        if ((i & 255) == 0 && c.dead) return false;
+        uint32_t done;
+        asm volatile("{\n\t.reg .pred p;\n\t"
+                     "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+                     "selp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+        if (done) return true;
+    }
+    c.dead = 1;
+    atomicOr(err, WC_ERR_TMA_WAIT);
+    return false;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
+{
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_commit(uint64_t *bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+}
+/* Shared-memory operand: start address, leading and stride offsets in bytes,
+ * swizzle 128 B (2) or 64 B (4). */
+__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t swizzle)
+{
+    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 |
+           (uint64_t)((sbo >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void bar_named(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
+
+template <int NC> __device__ __forceinline__ void tm_ld(float *v, uint32_t addr)
+{
+    uint32_t *u = reinterpret_cast<uint32_t *>(v);
+#pragma unroll
+    for (int k = 0; k < NC; k += 16)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                     "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : "=r"(u[k]), "=r"(u[k + 1]), "=r"(u[k + 2]), "=r"(u[k + 3]), "=r"(u[k + 4]),
+                       "=r"(u[k + 5]), "=r"(u[k + 6]), "=r"(u[k + 7]), "=r"(u[k + 8]), "=r"(u[k + 9]),
+                       "=r"(u[k + 10]), "=r"(u[k + 11]), "=r"(u[k + 12]), "=r"(u[k + 13]),
+                       "=r"(u[k + 14]), "=r"(u[k + 15])
+                     : "r"(addr + k));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+template <int NC> __device__ __forceinline__ void tm_st(const float *v, uint32_t addr)
+{
+    const uint32_t *u = reinterpret_cast<const uint32_t *>(v);
+#pragma unroll
+    for (int k = 0; k < NC; k += 16)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+                     "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                     ::"r"(addr + k), "r"(u[k]), "r"(u[k + 1]), "r"(u[k + 2]), "r"(u[k + 3]), "r"(u[k + 4]),
+                       "r"(u[k + 5]), "r"(u[k + 6]), "r"(u[k + 7]), "r"(u[k + 8]), "r"(u[k + 9]),
+                       "r"(u[k + 10]), "r"(u[k + 11]), "r"(u[k + 12]), "r"(u[k + 13]),
+                       "r"(u[k + 14]), "r"(u[k + 15]) : "memory");
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+/* The largest of the 32 lanes' values, NaN left out, in every lane. */
+__device__ __forceinline__ float warp_max(float v)
+{
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b)
+{
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+/* Sums of NC values over the 32 lanes: lane l ends with that of column
+ * l % NC. */
+template <int NC> __device__ __forceinline__ float lane_sums(float *v, int lane)
+{
+    if (NC == 16) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+    }
+#pragma unroll
+    for (int o = NC / 2; o > 0; o >>= 1) {
+        const bool up = lane & o;
+#pragma unroll
+        for (int i = 0; i < o; i++) {
+            const float give = up ? v[i] : v[i + o];
+            const float got = __shfl_xor_sync(0xffffffffu, give, o);
+            v[i] = (up ? v[i + o] : v[i]) + got;
+        }
+    }
+    return v[0];
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_constant__ Shape p,
+                                                               const __grid_constant__ CUtensorMap map,
+                                                               int box_rows)
+{
+    using Cfg = TcCfg<N>;
+    constexpr int NC = Cfg::NC;
+    constexpr bool kF16 = sizeof(T) == 2 && std::is_same<T, __half>::value;
+    /* weights of fp16 are scaled up, so that small ones keep their bits */
+    constexpr float kBias = kF16 ? 8.0f : 0.0f;
+    extern __shared__ unsigned char smt[];
+    unsigned char *sm = smt + ((1024 - (smem_u32(smt) & 1023)) & 1023);
+    TcCtl &c = *reinterpret_cast<TcCtl *>(sm + Cfg::off_ctl);
+    const waste_cuda_mla_tree_desc &d = p.d;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int npair = d.kl / 128, nchunk = d.kl / 64 + (d.rope > 0), H = d.heads;
+
+    wc_pdl::trigger();
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+                     ::"r"(smem_u32(&c.tmem)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    if (tid == 0) {
+        p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+        for (int i = 0; i < Cfg::pairs; i++) { mbar_init(&c.pair_full[i], 1); mbar_init(&c.pair_empty[i], 1); }
+        mbar_init(&c.rope_full, 1);
+        mbar_init(&c.rope_empty, 1);
+        mbar_init(&c.q_full, 256);
+        mbar_init(&c.s_full, 1);
+        mbar_init(&c.p_ready, 256);
+        mbar_init(&c.o_done, 1);
+        mbar_init(&c.drain, 1);
+        c.dead = 0;
+        mbar_fence_init();
+    }
+    Walk w;
+    long long total;
+    const bool any = walk_begin(p, w, c.red, total);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;
+    Seg g;
+    if (any && warp == 0) {
+        /* ---- loads: a lane a box of box_rows keys ---- */
+        int it = 0;                                           /* pairs issued            */
+        int ur = 0;                                           /* rope chunks issued      */
+        while (walk_next(p, w, g)) {
+            for (int kt = g.k0; kt < g.k1; kt++) {
+                const int k0 = kt * kTcKeys, nk = min(kTcKeys, g.vis - k0);
+                const int nbox = (nk + box_rows - 1) / box_rows;
+                int blk = 0, row = 0;
+                if (lane < nbox) {
+                    const int key = k0 + lane * box_rows, b = key / d.page;
+                    row = key - b * d.page;
+                    blk = d.block_table[(size_t)g.q.r * d.max_blocks + b];
+                    if (blk < 0 || blk >= d.n_blocks) {
+                        atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+                        blk = (int)d.n_blocks;              /* reads zeros */
+                    }
+                }
+                const uint32_t chunk_tx = (uint32_t)(nbox * box_rows) * 128u;
+                for (int j = 0; j <= npair; j++) {
+                    const bool rope = j == npair;
+                    if (rope && d.rope == 0) continue;
+                    uint64_t *full = rope ? &c.rope_full : &c.pair_full[it % Cfg::pairs];
+                    uint64_t *empty = rope ? &c.rope_empty : &c.pair_empty[it % Cfg::pairs];
+                    const int use = rope ? ur : it / Cfg::pairs;
+                    bool ok = true;
+                    if (use > 0) ok = tc_wait(c, empty, (use - 1) & 1, p.err);
+                    ok = __all_sync(0xffffffffu, ok && !c.dead);
+                    if (!ok) continue;
+                    if (lane == 0) mbar_expect_tx(full, rope ? chunk_tx : 2 * chunk_tx);
+                    __syncwarp();
+                    if (lane < nbox) {
+                        unsigned char *dst = sm + (rope ? Cfg::off_rope : (it % Cfg::pairs) * kPairBytes) +
+                                             lane * box_rows * 128;
+                        tma_load_3d(dst, &map, j * 128, row, blk, full);
+                        if (!rope) tma_load_3d(dst + kTcKeys * 128, &map, j * 128 + 64, row, blk, full);
+                    }
+                    if (rope) ur++; else it++;
+                }
+            }
+        }
+        if (c.dead) {                                         /* what is in flight lands */
+            for (int i = 0; i < Cfg::pairs; i++)
+                if (it > i) mbar_wait(&c.pair_full[i], ((it - 1 - i) / Cfg::pairs) & 1);
+            if (ur > 0) mbar_wait(&c.rope_full, (ur - 1) & 1);
+        }
+    } else if (any && warp == 1) {
+        if (lane == 0) {
+            /* ---- products ---- */
+            const uint32_t fmt = kF16 ? 0u : 1u;
+            const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
+            const uint32_t id_s = base, id_o = base | (1u << 15) | (1u << 16);
+            const uint32_t sq = smem_u32(sm + Cfg::off_q), sp = smem_u32(sm + Cfg::off_p);
+            const uint32_t sr = smem_u32(sm + Cfg::off_rope);
+            const int rope_steps = (d.rope + 15) / 16;
+            int it = 0, unit = 0, segs = 0;
+            while (walk_next(p, w, g)) {
+                if (g.k0 == g.k1) continue;
+                tc_wait(c, &c.q_full, segs & 1, p.err);
+                for (int kt = g.k0; kt < g.k1; kt++, unit++) {
+                    tc_fence_after();
+                    for (int j = 0; j < npair; j++) {
+                        const int slot = (it + j) % Cfg::pairs;
+                        tc_wait(c, &c.pair_full[slot], ((it + j) / Cfg::pairs) & 1, p.err);
+                        if (c.dead) break;
+                        tc_fence_after();
+                        const uint32_t a = smem_u32(sm + slot * kPairBytes), b = sq + j * 2 * N * 128;
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            tc_mma(tm_s, tc_desc(a + (k >> 2) * kTcKeys * 128 + (k & 3) * 32, 16, 1024, 2),
+                                   tc_desc(b + (k >> 2) * N * 128 + (k & 3) * 32, 16, 1024, 2), id_s,
+                                   j > 0 || k > 0);
+                    }
+                    if (d.rope > 0) {
+                        tc_wait(c, &c.rope_full, unit & 1, p.err);
+                        tc_fence_after();
+                        for (int k = 0; k < rope_steps && !c.dead; k++)
+                            tc_mma(tm_s, tc_desc(sr + k * 32, 16, 1024, 2),
+                                   tc_desc(sq + npair * 2 * N * 128 + k * 32, 16, 1024, 2), id_s, 1u);
+                    }
+                    if (!c.dead) {
+                        tc_commit(&c.s_full);
+                        if (N != 64) tc_commit(&c.rope_empty);
+                    }
+                    tc_wait(c, &c.p_ready, unit & 1, p.err);
+                    tc_fence_after();
+                    for (int j = 0; j < npair && !c.dead; j++) {
+                        const int slot = (it + j) % Cfg::pairs;
+                        const uint32_t a = smem_u32(sm + slot * kPairBytes);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            tc_mma(tmem + j * N, tc_desc(a + k * 2048, kTcKeys * 128, 1024, 2),
+                                   tc_desc(sp + k * 16 * Cfg::p_row, 16, 8 * Cfg::p_row, N == 64 ? 2 : 4),
+                                   id_o, kt > g.k0 || k > 0);
+                        tc_commit(&c.pair_empty[slot]);
+                    }
+                    if (N == 64 && !c.dead) tc_commit(&c.rope_empty);
+                    it += npair;
+                }
+                if (!c.dead) tc_commit(&c.o_done);
+                segs++;
+            }
+            if (c.dead) {                                     /* the products in flight end */
+                tc_commit(&c.drain);
+                mbar_wait(&c.drain, 0);
+            }
+        }
+        __syncwarp();
+    } else if (any && warp >= 2) {
+        /* ---- softmax ---- */
+        const int st = tid - 64, half = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = half * NC;
+        const uint32_t tm_lane = (uint32_t)(quad * 32) << 16;
+        const float scale2 = d.scale * 1.4426950408889634f;
+        float *mine = c.col[warp - 2];
+        int unit = 0, it = 0, segs = 0;
+        while (walk_next(p, w, g)) {
+            const bool whole = g.first && g.last;
+            const int slot = part_slot(g);
+            float l[NC];
+            float ref = -INFINITY;                            /* of column c0 + lane        */
+#pragma unroll
+            for (int i = 0; i < NC; i++) l[i] = 0.0f;
+            if (g.k0 < g.k1) {
+                /* the query tile: swizzled 128-byte rows, zeros past its rows and columns */
+                const int D = d.kl + d.rope, per = nchunk * 8;
+                for (int i = st; i < N * per; i += 256) {
+                    const int row = i / per, u = i - row * per, col = u * 8, at = g.row0 + row;
+                    uint4 v = make_uint4(0, 0, 0, 0);
+                    if (row < g.rows && col < D)
+                        v = __ldg(reinterpret_cast<const uint4 *>(
+                            static_cast<const T *>(d.q) + (size_t)(g.q.q0 + at / H) * d.q_token_stride +
+                            (size_t)(at % H) * d.q_head_stride + col));
+                    *reinterpret_cast<uint4 *>(sm + Cfg::off_q + (u >> 3) * N * 128 + row * 128 +
+                                               (((u & 7) ^ (row & 7)) << 4)) = v;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                mbar_arrive(&c.q_full);
+            }
+            for (int kt = g.k0; kt < g.k1; kt++, unit++, it += npair) {
+                const int key = kt * kTcKeys + key_row;
+                const bool tail = kt * kTcKeys + kTcKeys > g.q.ctx || kt * kTcKeys + kTcKeys > g.vis;
+                float x[NC];
+                tc_wait(c, &c.s_full, unit & 1, p.err);
+                tc_fence_after();
+                tm_ld<NC>(x, tm_s + tm_lane + c0);
+#pragma unroll
+                for (int i = 0; i < NC; i++) x[i] *= scale2;
+                if (tail) {
+                    /* rows past the request's are zeros to the second product, and so is
+                     * a new row that holds a NaN or an infinity: who sees it gets NaN
+                     * weights, who does not is not touched */
+                    for (int j = 0; j < npair; j++)
+                        tc_wait(c, &c.pair_full[(it + j) % Cfg::pairs], ((it + j) / Cfg::pairs) & 1, p.err);
+                    if (half == 0) c.nan_row[key_row] = 0;
+                    bar_named(3, 256);
+                    if (key >= g.q.ctx && key < g.vis) {
+                        bool bad = false;
+                        for (int j = half; j < npair; j += 2) {
+                            const unsigned char *b = sm + ((it + j) % Cfg::pairs) * kPairBytes + key_row * 128;
+                            for (int u = 0; u < 16; u++) {
+                                const uint4 v = *reinterpret_cast<const uint4 *>(
+                                    b + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4));
+                                const uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u;
+                                bad |= __vcmpeq2(v.x & e, e) || __vcmpeq2(v.y & e, e) || __vcmpeq2(v.z & e, e) ||
+                                       __vcmpeq2(v.w & e, e);
+                            }
+                        }
+                        if (bad) c.nan_row[key_row] = 1;
+                    }
+                    bar_named(3, 256);
+                    const bool bad = c.nan_row[key_row];
+                    if (bad || key >= g.vis) {
+                        for (int j = half; j < npair; j += 2) {
+                            unsigned char *b = sm + ((it + j) % Cfg::pairs) * kPairBytes + key_row * 128;
+                            for (int u = 0; u < 16; u++)
+                                *reinterpret_cast<uint4 *>(b + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4)) =
+                                    make_uint4(0, 0, 0, 0);
+                        }
+                    }
+                    int tok = (g.row0 + c0) / H, h = g.row0 + c0 - tok * H;
+                    bool see = key < g.vis && (key < g.q.ctx || (tok < g.q.n && sees(p, g.q, tok, key - g.q.ctx)));
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        if (!see) x[i] = -INFINITY;
+                        else if (bad) x[i] = __int_as_float(0x7fc00000);
+                        if (++h == H) {
+                            h = 0;
+                            tok++;
+                            see = key < g.vis && (key < g.q.ctx || (tok < g.q.n && sees(p, g.q, tok, key - g.q.ctx)));
+                        }
+                    }
+                }
+                /* the columns' maxima over the tile's 128 keys */
+                float mx = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const float m = warp_max(x[i]);
+                    if (lane == i) mx = m;
+                }
+                float (*sx)[32] = c.mx[unit & 1][half];
+                if (lane < NC) sx[quad][lane] = mx;
+                bar_named(1 + half, 128);
+                const int lc = lane % NC;
+                mx = fmaxf(fmaxf(sx[0][lc], sx[1][lc]), fmaxf(sx[2][lc], sx[3][lc]));
+                const bool grow = mx > ref + kLazy;           /* also at the first finite one */
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float a = grow ? (ref == -INFINITY ? 0.0f : ex2(ref - mx)) : 1.0f;
+                    if (grow) ref = mx;
+                    __syncwarp();
+                    if (lane < NC) mine[lane] = a;
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < NC; i++) l[i] *= mine[i];
+                    if (kt > g.k0) {
+                        /* the products before are done: S's commit followed them */
+                        for (int j = 0; j < npair; j++) {
+                            float o[NC];
+                            tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
+#pragma unroll
+                            for (int i = 0; i < NC; i++) o[i] *= mine[i];
+                            tm_st<NC>(o, tmem + tm_lane + j * N + c0);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane < NC) mine[lane] = (ref == -INFINITY ? 0.0f : ref) - kBias;
+                __syncwarp();
+                uint32_t pk[NC / 2];
+#pragma unroll
+                for (int i = 0; i < NC; i += 2) {
+                    const float e0 = ex2(x[i] - mine[i]), e1 = ex2(x[i + 1] - mine[i + 1]);
+                    l[i] += e0;
+                    l[i + 1] += e1;
+                    pk[i / 2] = pack2<T>(e0, e1);
+                }
+                unsigned char *pr = sm + Cfg::off_p + key_row * Cfg::p_row;
+                const int sw = N == 64 ? key_row & 7 : (key_row >> 1) & 3;
+#pragma unroll
+                for (int u = 0; u < NC / 8; u++)
+                    *reinterpret_cast<uint4 *>(pr + (((c0 / 8 + u) ^ sw) << 4)) =
+                        make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_fence_before();
+                mbar_arrive(&c.p_ready);
+            }
+            /* ---- the segment's result ---- */
+            float sum = lane_sums<NC>(l, lane);               /* of column lane % NC         */
+            float (*sx)[32] = c.mx[unit & 1][half];
+            if (lane < NC) sx[quad][lane] = sum;
+            bar_named(1 + half, 128);
+            const int lc = lane % NC;
+            sum = (sx[0][lc] + sx[1][lc]) + (sx[2][lc] + sx[3][lc]);
+            bar_named(1 + half, 128);                         /* read before it is reused    */
+            const float m = (ref == -INFINITY ? 0.0f : ref) - kBias;
+            __syncwarp();
+            if (lane < NC) mine[lane] = sum == 0.0f ? 0.0f : 1.0f / sum;
+            __syncwarp();
+            const int row = c0 + lane;
+            if (quad == 0 && lane < NC && row < g.rows) {
+                if (whole) {
+                    if (d.lse)
+                        d.lse[(size_t)g.q.q0 * H + g.row0 + row] =
+                            sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.693147180559945f;
+                } else {
+                    p.stat[((size_t)slot * N + row) * 2] = sum == 0.0f ? -INFINITY : m;
+                    p.stat[((size_t)slot * N + row) * 2 + 1] = sum;
+                }
+            }
+            const bool some = g.k0 < g.k1;
+            if (some) {
+                tc_wait(c, &c.o_done, segs & 1, p.err);
+                tc_fence_after();
+                segs++;
+            }
+            if (some || whole) {
+                for (int j = 0; j < npair; j++) {
+                    float o[NC];
+                    if (some) tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
+                    const int cd = j * 128 + key_row;
+                    int tok = (g.row0 + c0) / H, h = g.row0 + c0 - tok * H;
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        if (c0 + i < g.rows) {
+                            if (whole) {
+                                const float inv = mine[i];
+                                static_cast<T *>(d.o)[(size_t)(g.q.q0 + tok) * d.o_token_stride +
+                                                      (size_t)h * d.o_head_stride + cd] =
+                                    from_f<T>(inv == 0.0f || !some ? 0.0f : o[i] * inv);
+                            } else {
+                                p.part[((size_t)slot * N + c0 + i) * d.kl + cd] = o[i];
+                            }
+                        }
+                        if (++h == H) { h = 0; tok++; }
+                    }
+                }
+            }
+            tc_fence_before();
+            if (st == 0) note_split(p, g, total);
+        }
+    }
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+}
+
 /* ---- split tiles joined ------------------------------------------------------
  * grid (CTAs of the attention, rows of a tile): the tile whose first units
  * CTA c held, one row. o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s over
@@ -485,21 +1007,67 @@ cudaError_t gen_launch(Shape &p, int sms, cudaStream_t s)
     return e;
 }
 
+template <typename T, int N>
+cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, cudaStream_t s)
+{
+    p.NT = N;
+    p.KT = kTcKeys;
+    carve(&p, sms);
+    const size_t smem = TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024;
+    static_assert(TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024 <= 227 * 1024, "attention tile exceeds shared memory");
+    cudaError_t e = cudaFuncSetAttribute(mla_tc_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         (int)smem);
+    if (e != cudaSuccess) return e;
+    mla_tc_kernel<T, N><<<sms, kTcThreads, smem, s>>>(p, map, box_rows);
+    wc_count_launches(1);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    e = wc_pdl::launch(mla_combine_kernel<T, 1>, dim3(sms, N), dim3(kCombThreads), 0, s, true, p);
+    wc_count_launches(1);
+    return e;
+}
+
+template <typename T>
+cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, cudaStream_t s)
+{
+    return (long long)p.d.T * p.d.heads <= 32ll * p.d.B ? tc_launch<T, 32>(p, map, box_rows, sms, s)
+                                                        : tc_launch<T, 64>(p, map, box_rows, sms, s);
+}
+
 } /* namespace */
 
 extern "C" {
+
+/* Whether the tensor-core kernel takes the call: a 16-bit cache of whole
+ * 128-column pairs and a rope part of at most a chunk, pages of whole 8-row
+ * swizzle groups, and rows TMA and 16-byte loads can start at. Its boxes are
+ * 64 columns by the returned number of rows (0: the other kernel's). */
+int wc_mla_tree_box(const waste_cuda_mla_tree_desc *d)
+{
+    const uintptr_t addr = (uintptr_t)d->q | (uintptr_t)d->cache;
+    if (d->dtype == WASTE_CUDA_F32 || d->kl % 128 || d->rope > 64 || d->rope % 8 || d->page % 8 || (addr & 15) ||
+        d->row_stride % 8 || d->q_token_stride % 8 || d->q_head_stride % 8 || d->n_blocks < 1 ||
+        d->n_blocks > 0x7fffffff || d->row_stride * 2 * d->page >= ((size_t)1 << 40))
+        return 0;
+    int r = 8;
+    while (r < kTcKeys && d->page % (2 * r) == 0) r *= 2;
+    return r;
+}
 
 size_t wc_mla_tree_ws_bytes(int kl, int sms)
 {
     return (size_t)2 * sms * kTileMax * (kl + 2) * sizeof(float) + (size_t)sms * sizeof(int4);
 }
 
-int wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, unsigned int *err, int sms, void *stream)
+int wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *map, int box_rows,
+                       unsigned int *err, int sms, void *stream)
 {
     Shape p = {};
     p.d = *d;
     p.err = err;
     const cudaStream_t s = (cudaStream_t)stream;
+    if (box_rows > 0)
+        return (int)(d->dtype == WASTE_CUDA_F16 ? tc_launch<__half>(p, *map, box_rows, sms, s)
+                                                : tc_launch<__nv_bfloat16>(p, *map, box_rows, sms, s));
     if (d->dtype == WASTE_CUDA_F32) return (int)gen_launch<float>(p, sms, s);
     if (d->dtype == WASTE_CUDA_F16) return (int)gen_launch<__half>(p, sms, s);
     return (int)gen_launch<__nv_bfloat16>(p, sms, s);

@@ -3394,8 +3394,27 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
                   wc_mla_tree_ws_bytes(d->kl, S.sms));
         goto out;
     }
-    CK((cudaError_t)wc_mla_tree_launch(d, S.d_serr, S.sms, stream ? stream : (void *)S.stream),
-       "mla_tree_attn");
+    int box = wc_mla_tree_box(d);
+    CUtensorMap map;
+    if (box) {
+        const cuuint64_t dims[3] = { (cuuint64_t)(d->kl + d->rope), (cuuint64_t)d->page,
+                                     (cuuint64_t)d->n_blocks };
+        const cuuint64_t strides[2] = { d->row_stride * z, d->row_stride * z * (size_t)d->page };
+        const cuuint32_t tile[3] = { 64, (cuuint32_t)box, 1 }, estr[3] = { 1, 1, 1 };
+        wc_encode_tiled_fn enc = encode_tiled();
+        if (!enc || enc(&map,
+                        d->dtype == WASTE_CUDA_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                        3, (void *)d->cache, dims, strides, tile, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS) {
+            rc = fail(WASTE_CUDA_E_DEVICE, "mla_tree_attn_dev: no tensor map of the cache");
+            goto out;
+        }
+    }
+    CK((cudaError_t)wc_mla_tree_launch(d, &map, box, S.d_serr, S.sms,
+                                       stream ? stream : (void *)S.stream), "mla_tree_attn");
 out:
     pthread_mutex_unlock(&g_mu);
     return rc;
