@@ -58,12 +58,18 @@ struct Req {
 
 struct Shape {
     waste_cuda_mla_tree_desc d;
-    int NT, KT;
+    int NT, KT, kt_log;              /* KT = 1 << kt_log                         */
     unsigned int *err;
     float *part;                     /* [2 * grid][NT][kl] partial sums          */
     float *stat;                     /* [2 * grid][NT][2] their maxima and sums  */
     int4 *meta;                      /* [grid] the tile that starts to be split there */
 };
+
+/* 64-bit quotients cost a few hundred cycles, and most here fit 32 bits */
+__device__ __forceinline__ unsigned long long div_u(unsigned long long a, unsigned long long b)
+{
+    return ((a | b) >> 32) ? a / b : (unsigned long long)((unsigned)a / (unsigned)b);
+}
 
 __device__ __forceinline__ Req req_at(const Shape &p, int r)
 {
@@ -78,37 +84,37 @@ __device__ __forceinline__ Req req_at(const Shape &p, int r)
     if (q.bad) kv = (int)cap;
     q.kv = kv < q.n ? 0 : kv;
     q.ctx = q.kv - (q.kv ? q.n : 0);
-    q.nt = (int)(((long long)q.n * d.heads + p.NT - 1) / p.NT);
+    q.nt = (int)(((unsigned)q.n * (unsigned)d.heads + p.NT - 1u) / (unsigned)p.NT);
     return q;
 }
 
 __device__ __forceinline__ long long unit_prefix(const Shape &p, const Req &q, int i)
 {
     if (!p.d.mask && q.nt > 1 && q.kv) {
-        const long long H2 = 2ll * p.d.heads;
-        return (H2 * i * (q.ctx + 1ll) + (long long)p.NT * i * (i + 1ll)) / (H2 * p.KT) + i;
+        const unsigned H2 = 2u * p.d.heads;
+        return (long long)(div_u(H2 * i * (q.ctx + 1ull) + (unsigned long long)p.NT * i * (i + 1ull), H2) >> p.kt_log) + i;
     }
-    return (long long)i * max(1, (q.kv + p.KT - 1) / p.KT);
+    return (long long)i * max(1, (q.kv + p.KT - 1) >> p.kt_log);
 }
 
 /* One CTA's share of one query tile: key tiles [k0, k1). */
 struct Seg {
     Req q;
-    int tile, k0, k1;
+    int k0, k1;
     int vis;                         /* keys the tile's last row sees             */
     bool first, last;                /* the tile's units all before / behind are here */
-    long long units;                 /* nominal units of this segment             */
     int row0, rows;                  /* rows of the request                       */
     long long tile_u0, tile_u1;      /* the tile's units, global                  */
 };
 
 struct Walk {
-    long long u, u1, base;           /* next unit, end, the request's first unit  */
-    int r;
+    long long u, u1;                 /* next unit, end                            */
+    long long base, tile_u0;         /* first unit of the request, of the tile    */
+    int r, tile;
     Req q;
 };
 
-/* All threads: the CTA's range of units and where it starts. `red` holds 66
+/* All threads: the CTA's range of units and where it starts. `red` holds 67
  * long longs of shared memory. Returns false when the range is empty. */
 __device__ bool walk_begin(const Shape &p, Walk &w, long long *red, long long &total)
 {
@@ -136,13 +142,23 @@ __device__ bool walk_begin(const Shape &p, Walk &w, long long *red, long long &t
     total = all;
     /* with fewer units than CTAs, the first CTAs take one each */
     const long long G = max(1ll, min((long long)gridDim.x, all)), c = blockIdx.x;
-    w.u = c < G ? c * all / G : all;
-    w.u1 = c < G ? (c + 1) * all / G : all;
+    w.u = c < G ? (long long)div_u(c * all, G) : all;
+    w.u1 = c < G ? (long long)div_u((c + 1) * all, G) : all;
     if (sum > 0 && at <= w.u && w.u < at + sum) {
         for (int k = 0; k < per && r0 + k < p.d.B; k++) {
             const Req q = req_at(p, r0 + k);
             const long long n = unit_prefix(p, q, q.nt);
-            if (w.u < at + n) { red[64] = r0 + k; red[65] = at; break; }
+            if (w.u < at + n) {
+                int lo = 0, hi = q.nt;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (at + unit_prefix(p, q, mid) <= w.u) lo = mid; else hi = mid;
+                }
+                red[64] = r0 + k;
+                red[65] = at;
+                red[66] = lo;
+                break;
+            }
             at += n;
         }
     }
@@ -150,36 +166,32 @@ __device__ bool walk_begin(const Shape &p, Walk &w, long long *red, long long &t
     if (w.u >= w.u1) return false;
     w.r = (int)red[64];
     w.base = red[65];
+    w.tile = (int)red[66];
     w.q = req_at(p, w.r);
+    w.tile_u0 = w.base + unit_prefix(p, w.q, w.tile);
     return true;
 }
 
 __device__ __forceinline__ bool walk_next(const Shape &p, Walk &w, Seg &s)
 {
     if (w.u >= w.u1) return false;
-    long long n = unit_prefix(p, w.q, w.q.nt);
-    while (w.u >= w.base + n) {
-        w.base += n;
+    while (w.tile == w.q.nt) {
+        w.base = w.tile_u0;
         w.q = req_at(p, ++w.r);
-        n = unit_prefix(p, w.q, w.q.nt);
+        w.tile = 0;
     }
-    int lo = 0, hi = w.q.nt;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (w.base + unit_prefix(p, w.q, mid) <= w.u) lo = mid; else hi = mid;
-    }
+    const int lo = w.tile++;
     const int H = p.d.heads;
     s.q = w.q;
-    s.tile = lo;
-    s.tile_u0 = w.base + unit_prefix(p, w.q, lo);
-    s.tile_u1 = w.base + unit_prefix(p, w.q, lo + 1);
+    s.tile_u0 = w.tile_u0;
+    s.tile_u1 = w.tile_u0 = w.base + unit_prefix(p, w.q, lo + 1);
     const long long end = min(s.tile_u1, w.u1);
     s.first = w.u == s.tile_u0;
     s.last = end == s.tile_u1;
     s.row0 = lo * p.NT;
     s.rows = min(p.NT, w.q.n * H - s.row0);
     s.vis = p.d.mask || !w.q.kv ? w.q.kv : min(w.q.kv, w.q.ctx + (s.row0 + s.rows - 1) / H + 1);
-    const int kt = (s.vis + p.KT - 1) / p.KT;
+    const int kt = (s.vis + p.KT - 1) >> p.kt_log;
     s.k0 = (int)min((long long)kt, w.u - s.tile_u0);
     s.k1 = (int)min((long long)kt, end - s.tile_u0);
     w.u = end;
@@ -203,7 +215,7 @@ __device__ __forceinline__ int part_slot(const Seg &s) { return 2 * blockIdx.x +
 __device__ __forceinline__ void note_split(const Shape &p, const Seg &s, long long total)
 {
     if (s.first && !s.last) {
-        const long long G = min((long long)gridDim.x, total), c1 = (s.tile_u1 * G - 1) / total;
+        const long long G = min((long long)gridDim.x, total), c1 = (long long)div_u(s.tile_u1 * G - 1, total);
         p.meta[blockIdx.x] = make_int4(s.q.q0 * p.d.heads + s.row0, s.rows, (int)c1, 1);
     }
 }
@@ -226,7 +238,7 @@ struct GenSmem {
     float p[kGenKeys][kGenRows];     /* scores, then weights                      */
     float m[kGenRows], l[kGenRows], a[kGenRows];
     long long off[kGenKeys];         /* element offset of a key's row, -1: none   */
-    long long red[66];
+    long long red[67];
 };
 
 template <typename T>
@@ -459,22 +471,24 @@ struct TcCtl {
     uint64_t rope_full, rope_empty, q_full, s_full, p_ready, o_done, drain;
     uint32_t tmem;
     volatile int dead;
-    long long red[66];
+    long long red[67];
     float mx[2][2][4][32];           /* [parity][half][quadrant][column] maxima     */
     float col[8][32];                /* a warp's broadcast of one value a column     */
+    long long qoff[64], ooff[64];    /* a tile row's elements in q (-1: no row) and o */
+    int tok[64];                     /* its token in the request                     */
     unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
 };
 
 __device__ __forceinline__ bool tc_wait(TcCtl &c, uint64_t *bar, uint32_t parity, unsigned int *err)
 {
     for (int i = 0; i < kMbarLimit; i++) {
-        if ((i & 255) == 0 && c.dead) return false;
         uint32_t done;
         asm volatile("{\n\t.reg .pred p;\n\t"
                      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
                      "selp.u32 %0, 1, 0, p;\n\t}"
                      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
         if (done) return true;
+        if (c.dead) return false;
     }
     c.dead = 1;
     atomicOr(err, WC_ERR_TMA_WAIT);
@@ -485,23 +499,33 @@ __device__ __forceinline__ void mbar_arrive(uint64_t *bar)
 {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+__device__ __forceinline__ bool elect()
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void tc_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
                  ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+/* Shared-memory operand descriptors: the low word has the start address and
+ * the leading offset, the high word the stride offset, version 1 and the
+ * swizzle (128 B: 2, 64 B: 4); offsets in bytes. */
+__device__ __forceinline__ uint32_t desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | (lbo >> 4) << 16; }
+__host__ __device__ constexpr uint32_t desc_hi(uint32_t sbo, uint32_t swizzle)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}\n"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+    return (sbo >> 4) | 1u << 14 | swizzle << 29;
 }
-/* Shared-memory operand: start address, leading and stride offsets in bytes,
- * swizzle 128 B (2) or 64 B (4). */
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo, uint32_t swizzle)
+template <uint32_t AHI, uint32_t BHI>
+__device__ __forceinline__ void tc_mma(uint32_t d, uint32_t alo, uint32_t blo, uint32_t idesc, uint32_t acc)
 {
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((lbo >> 4) & 0x3fff) << 16 |
-           (uint64_t)((sbo >> 4) & 0x3fff) << 32 | (uint64_t)1 << 46 | (uint64_t)swizzle << 61;
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+                 "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %6};\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}\n"
+                 ::"r"(d), "r"(alo), "r"(blo), "r"(idesc), "r"(acc), "n"(AHI), "n"(BHI) : "memory");
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -623,7 +647,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;
+    const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;            /* O | S^T */
     Seg g;
     if (any && warp == 0) {
         /* ---- loads: a lane a box of box_rows keys ---- */
@@ -672,62 +696,67 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
             if (ur > 0) mbar_wait(&c.rope_full, (ur - 1) & 1);
         }
     } else if (any && warp == 1) {
-        if (lane == 0) {
-            /* ---- products ---- */
-            const uint32_t fmt = kF16 ? 0u : 1u;
-            const uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
-            const uint32_t id_s = base, id_o = base | (1u << 15) | (1u << 16);
-            const uint32_t sq = smem_u32(sm + Cfg::off_q), sp = smem_u32(sm + Cfg::off_p);
-            const uint32_t sr = smem_u32(sm + Cfg::off_rope);
+        /* ---- products: one lane ---- */
+        if (elect()) {
+            constexpr uint32_t fmt = kF16 ? 0u : 1u;
+            constexpr uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
+            constexpr uint32_t id_o = id_s | (1u << 15) | (1u << 16);
+            constexpr uint32_t kHi = desc_hi(1024, 2), kHiP = desc_hi(8 * Cfg::p_row, N == 64 ? 2 : 4);
+            const uint32_t sm0 = smem_u32(sm);
+            const uint32_t k_lo = desc_lo(sm0, 16), v_lo = desc_lo(sm0, kTcKeys * 128);
+            const uint32_t q_lo = desc_lo(sm0 + Cfg::off_q, 16), p_lo = desc_lo(sm0 + Cfg::off_p, 16);
+            const uint32_t r_lo = desc_lo(sm0 + Cfg::off_rope, 16);
             const int rope_steps = (d.rope + 15) / 16;
-            int it = 0, unit = 0, segs = 0;
-            while (walk_next(p, w, g)) {
+            int slot0 = 0, par0 = 0;                          /* the tile's first pair       */
+            int unit = 0, segs = 0;
+            bool ok = true;
+            while (ok && walk_next(p, w, g)) {
                 if (g.k0 == g.k1) continue;
-                tc_wait(c, &c.q_full, segs & 1, p.err);
-                for (int kt = g.k0; kt < g.k1; kt++, unit++) {
+                ok = tc_wait(c, &c.q_full, segs & 1, p.err);
+                for (int kt = g.k0; kt < g.k1 && ok; kt++, unit++) {
+                    int slot = slot0, par = par0;
                     tc_fence_after();
+                    for (int j = 0; j < npair && ok; j++) {
+                        ok = tc_wait(c, &c.pair_full[slot], par, p.err);
+                        if (!ok) break;
+                        const uint32_t a = k_lo + slot * (kPairBytes / 16), b = q_lo + j * (2 * N * 128 / 16);
+#pragma unroll
+                        for (int k = 0; k < 8; k++)
+                            tc_mma<kHi, kHi>(tm_s, a + (k >> 2) * (kTcKeys * 128 / 16) + (k & 3) * 2,
+                                             b + (k >> 2) * (N * 128 / 16) + (k & 3) * 2, id_s, (j | k) != 0);
+                        if (++slot == Cfg::pairs) { slot = 0; par ^= 1; }
+                    }
+                    if (d.rope > 0 && ok) {
+                        ok = tc_wait(c, &c.rope_full, unit & 1, p.err);
+                        if (!ok) break;
+                        const uint32_t b = q_lo + npair * (2 * N * 128 / 16);
+                        for (int k = 0; k < rope_steps; k++)
+                            tc_mma<kHi, kHi>(tm_s, r_lo + k * 2, b + k * 2, id_s, 1u);
+                    }
+                    if (!ok) break;
+                    tc_commit(&c.s_full);
+                    if (N != 64) tc_commit(&c.rope_empty);
+                    ok = tc_wait(c, &c.p_ready, unit & 1, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    slot = slot0;
                     for (int j = 0; j < npair; j++) {
-                        const int slot = (it + j) % Cfg::pairs;
-                        tc_wait(c, &c.pair_full[slot], ((it + j) / Cfg::pairs) & 1, p.err);
-                        if (c.dead) break;
-                        tc_fence_after();
-                        const uint32_t a = smem_u32(sm + slot * kPairBytes), b = sq + j * 2 * N * 128;
+                        const uint32_t a = v_lo + slot * (kPairBytes / 16);
 #pragma unroll
                         for (int k = 0; k < 8; k++)
-                            tc_mma(tm_s, tc_desc(a + (k >> 2) * kTcKeys * 128 + (k & 3) * 32, 16, 1024, 2),
-                                   tc_desc(b + (k >> 2) * N * 128 + (k & 3) * 32, 16, 1024, 2), id_s,
-                                   j > 0 || k > 0);
-                    }
-                    if (d.rope > 0) {
-                        tc_wait(c, &c.rope_full, unit & 1, p.err);
-                        tc_fence_after();
-                        for (int k = 0; k < rope_steps && !c.dead; k++)
-                            tc_mma(tm_s, tc_desc(sr + k * 32, 16, 1024, 2),
-                                   tc_desc(sq + npair * 2 * N * 128 + k * 32, 16, 1024, 2), id_s, 1u);
-                    }
-                    if (!c.dead) {
-                        tc_commit(&c.s_full);
-                        if (N != 64) tc_commit(&c.rope_empty);
-                    }
-                    tc_wait(c, &c.p_ready, unit & 1, p.err);
-                    tc_fence_after();
-                    for (int j = 0; j < npair && !c.dead; j++) {
-                        const int slot = (it + j) % Cfg::pairs;
-                        const uint32_t a = smem_u32(sm + slot * kPairBytes);
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            tc_mma(tmem + j * N, tc_desc(a + k * 2048, kTcKeys * 128, 1024, 2),
-                                   tc_desc(sp + k * 16 * Cfg::p_row, 16, 8 * Cfg::p_row, N == 64 ? 2 : 4),
-                                   id_o, kt > g.k0 || k > 0);
+                            tc_mma<kHi, kHiP>(tmem + j * N, a + k * (2048 / 16), p_lo + k * (16 * Cfg::p_row / 16),
+                                              id_o, kt > g.k0 || k > 0);
                         tc_commit(&c.pair_empty[slot]);
+                        if (++slot == Cfg::pairs) slot = 0;
                     }
-                    if (N == 64 && !c.dead) tc_commit(&c.rope_empty);
-                    it += npair;
+                    if (N == 64) tc_commit(&c.rope_empty);
+                    slot0 += npair;
+                    if (slot0 >= Cfg::pairs) { slot0 -= Cfg::pairs; par0 ^= 1; }
                 }
-                if (!c.dead) tc_commit(&c.o_done);
+                if (ok) tc_commit(&c.o_done);
                 segs++;
             }
-            if (c.dead) {                                     /* the products in flight end */
+            if (!ok) {                                        /* the products in flight end */
                 tc_commit(&c.drain);
                 mbar_wait(&c.drain, 0);
             }
@@ -747,18 +776,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
             float ref = -INFINITY;                            /* of column c0 + lane        */
 #pragma unroll
             for (int i = 0; i < NC; i++) l[i] = 0.0f;
+            /* the tile's rows: where they are, once */
+            bar_named(3, 256);                                /* the last segment's are read */
+            if (st < N) {
+                const int at = g.row0 + st, tok = at / H, h = at - tok * H;
+                const bool in = st < g.rows;
+                c.tok[st] = in ? tok : 0x3fffffff;
+                c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * d.q_head_stride : -1;
+                c.ooff[st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
+            }
+            bar_named(3, 256);
             if (g.k0 < g.k1) {
-                /* the query tile: swizzled 128-byte rows, zeros past its rows and columns */
-                const int D = d.kl + d.rope, per = nchunk * 8;
-                for (int i = st; i < N * per; i += 256) {
-                    const int row = i / per, u = i - row * per, col = u * 8, at = g.row0 + row;
-                    uint4 v = make_uint4(0, 0, 0, 0);
-                    if (row < g.rows && col < D)
-                        v = __ldg(reinterpret_cast<const uint4 *>(
-                            static_cast<const T *>(d.q) + (size_t)(g.q.q0 + at / H) * d.q_token_stride +
-                            (size_t)(at % H) * d.q_head_stride + col));
-                    *reinterpret_cast<uint4 *>(sm + Cfg::off_q + (u >> 3) * N * 128 + row * 128 +
-                                               (((u & 7) ^ (row & 7)) << 4)) = v;
+                /* the query tile: swizzled 128-byte rows, zeros past its rows and columns;
+                 * 32 rows by a chunk's eight 16-byte units at a time */
+                const int D = d.kl + d.rope, u = st & 7;
+#pragma unroll
+                for (int rb = 0; rb < N; rb += 32) {
+                    const int row = rb + (st >> 3);
+                    const long long off = c.qoff[row];
+                    const T *src = static_cast<const T *>(d.q) + off + u * 8;
+                    unsigned char *dst = sm + Cfg::off_q + row * 128 + ((u ^ (row & 7)) << 4);
+                    uint4 v[9];
+#pragma unroll
+                    for (int k = 0; k < 9; k++)
+                        v[k] = off >= 0 && k < nchunk && k * 64 + u * 8 < D
+                                   ? __ldg(reinterpret_cast<const uint4 *>(src + k * 64)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int k = 0; k < 9; k++)
+                        if (k < nchunk) *reinterpret_cast<uint4 *>(dst + k * N * 128) = v[k];
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 mbar_arrive(&c.q_full);
@@ -804,17 +849,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                                     make_uint4(0, 0, 0, 0);
                         }
                     }
-                    int tok = (g.row0 + c0) / H, h = g.row0 + c0 - tok * H;
-                    bool see = key < g.vis && (key < g.q.ctx || (tok < g.q.n && sees(p, g.q, tok, key - g.q.ctx)));
+                    const int nj = key - g.q.ctx;             /* its place among the new rows */
+                    const bool in = key < g.vis;
+                    int last = -1;
+                    bool see = false;
 #pragma unroll
                     for (int i = 0; i < NC; i++) {
+                        const int tok = c.tok[c0 + i];
+                        if (tok != last) {
+                            last = tok;
+                            see = in && (nj < 0 || (tok < g.q.n && sees(p, g.q, tok, nj)));
+                        }
                         if (!see) x[i] = -INFINITY;
                         else if (bad) x[i] = __int_as_float(0x7fc00000);
-                        if (++h == H) {
-                            h = 0;
-                            tok++;
-                            see = key < g.vis && (key < g.q.ctx || (tok < g.q.n && sees(p, g.q, tok, key - g.q.ctx)));
-                        }
                     }
                 }
                 /* the columns' maxima over the tile's 128 keys */
@@ -900,24 +947,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 segs++;
             }
             if (some || whole) {
+                const int nc = min(NC, g.rows - c0);
+#pragma unroll 1
                 for (int j = 0; j < npair; j++) {
                     float o[NC];
                     if (some) tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
                     const int cd = j * 128 + key_row;
-                    int tok = (g.row0 + c0) / H, h = g.row0 + c0 - tok * H;
+                    if (whole) {
+                        T *dst = static_cast<T *>(d.o) + cd;
 #pragma unroll
-                    for (int i = 0; i < NC; i++) {
-                        if (c0 + i < g.rows) {
-                            if (whole) {
-                                const float inv = mine[i];
-                                static_cast<T *>(d.o)[(size_t)(g.q.q0 + tok) * d.o_token_stride +
-                                                      (size_t)h * d.o_head_stride + cd] =
-                                    from_f<T>(inv == 0.0f || !some ? 0.0f : o[i] * inv);
-                            } else {
-                                p.part[((size_t)slot * N + c0 + i) * d.kl + cd] = o[i];
-                            }
-                        }
-                        if (++h == H) { h = 0; tok++; }
+                        for (int i = 0; i < NC; i++)
+                            if (i < nc) dst[c.ooff[c0 + i]] = from_f<T>(some && mine[i] != 0.0f ? o[i] * mine[i] : 0.0f);
+                    } else {
+                        float *dst = p.part + ((size_t)slot * N + c0) * d.kl + cd;
+#pragma unroll
+                        for (int i = 0; i < NC; i++)
+                            if (i < nc) dst[(size_t)i * d.kl] = o[i];
                     }
                 }
             }
@@ -994,6 +1039,7 @@ cudaError_t gen_launch(Shape &p, int sms, cudaStream_t s)
 {
     p.NT = kGenRows;
     p.KT = kGenKeys;
+    p.kt_log = 6;
     carve(&p, sms);
     const size_t smem = sizeof(GenSmem) + (size_t)kGenRows * (p.d.kl + p.d.rope) * sizeof(float);
     cudaError_t e = cudaFuncSetAttribute(mla_gen_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1012,6 +1058,7 @@ cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, c
 {
     p.NT = N;
     p.KT = kTcKeys;
+    p.kt_log = 7;
     carve(&p, sms);
     const size_t smem = TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024;
     static_assert(TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024 <= 227 * 1024, "attention tile exceeds shared memory");
