@@ -135,9 +135,11 @@ __device__ bool walk_begin(const Shape &p, Walk &w, long long *red, long long &t
     if (lane == 31) red[warp] = inc;
     __syncthreads();
     long long at = inc - sum, all = 0;
-    for (int k = 0; k < nw; k++) {
-        if (k < warp) at += red[k];
-        all += red[k];
+#pragma unroll
+    for (int k = 0; k < 18; k++) {
+        const long long v = k < nw ? red[k] : 0;
+        if (k < warp) at += v;
+        all += v;
     }
     total = all;
     /* with fewer units than CTAs, the first CTAs take one each */
@@ -440,17 +442,19 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  * chunk was, which is read by then.
  *
  * Roles: warp 0 loads, one lane a box; a lane of warp 1 issues the products;
- * warps 2..9 do the softmax, a thread a key (TMEM lane) and half of the
- * columns: the column maxima by redux over the lanes and shared memory over
- * the 4 warps, the weights rounded and stored as P. The running maximum is
- * followed only when it grew by 2^kLazy or more (weights up to 2^kLazy are
- * exact powers away, the sums are 32 bits wide), so O in TMEM is rescaled a
- * few times at the start of a long row and hardly after.
+ * warps 2..17 do the softmax, a thread a key (TMEM lane) and a quarter of the
+ * columns. The weights are taken against a reference per column, an earlier
+ * tile's maximum, as long as none passes it by more than 2^kLazy (the 32-bit
+ * sums and the types' ranges allow that; the results are the same up to
+ * rounding): one vote a tile. Only where one does, at a row's start and a few
+ * times after, are the tile's maxima found (redux over the lanes, shared
+ * memory over the 4 warps), the reference moved and O in TMEM rescaled.
  *
  * Every wait is bounded: one that runs out raises WC_ERR_TMA_WAIT and
  * `dead`, upon which the roles run out their loops without waiting, issue
  * nothing more, and drain what is in flight. */
-constexpr int kTcThreads = 320;
+constexpr int kTcSoft = 512;          /* softmax threads */
+constexpr int kTcThreads = 64 + kTcSoft;
 constexpr int kTcKeys = 128;
 constexpr int kPairBytes = 2 * kTcKeys * 128;
 constexpr float kLazy = 6.0f;
@@ -458,7 +462,7 @@ constexpr int kMaxPairs = 5;
 
 template <int N> struct TcCfg {
     static constexpr int pairs = N == 64 ? 4 : 5;
-    static constexpr int NC = N / 2;                          /* columns a thread   */
+    static constexpr int NC = N / 4;                          /* columns a thread   */
     static constexpr int p_row = N * 2;                       /* bytes of a P row    */
     static constexpr int off_rope = pairs * kPairBytes;
     static constexpr int off_p = N == 64 ? off_rope : off_rope + kTcKeys * 128;
@@ -472,11 +476,14 @@ struct TcCtl {
     uint32_t tmem;
     volatile int dead;
     long long red[67];
-    float mx[2][2][4][32];           /* [parity][half][quadrant][column] maxima     */
-    float col[8][32];                /* a warp's broadcast of one value a column     */
+    float mx[4][4][16];              /* [quarter][quadrant][column]                  */
+    float col[16][2][16];            /* a warp's broadcast of values a column         */
     long long qoff[64], ooff[64];    /* a tile row's elements in q (-1: no row) and o */
     int tok[64];                     /* its token in the request                     */
     unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
+    Walk walk;                       /* the softmax warps' schedule, and their segment */
+    Seg seg;
+    int more;
 };
 
 __device__ __forceinline__ bool tc_wait(TcCtl &c, uint64_t *bar, uint32_t parity, unsigned int *err)
@@ -529,13 +536,21 @@ __device__ __forceinline__ void tc_mma(uint32_t d, uint32_t alo, uint32_t blo, u
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+/* a named barrier of 128 threads that also votes */
+__device__ __forceinline__ bool bar_any(int id, bool v)
+{
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\tbar.red.or.pred p, %1, 128, q;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"(id), "r"((uint32_t)v) : "memory");
+    return r != 0;
+}
 __device__ __forceinline__ void bar_named(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 template <int NC> __device__ __forceinline__ void tm_ld(float *v, uint32_t addr)
 {
     uint32_t *u = reinterpret_cast<uint32_t *>(v);
 #pragma unroll
-    for (int k = 0; k < NC; k += 16)
+    for (int k = 0; k + 16 <= NC; k += 16)
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
                      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                      : "=r"(u[k]), "=r"(u[k + 1]), "=r"(u[k + 2]), "=r"(u[k + 3]), "=r"(u[k + 4]),
@@ -543,19 +558,27 @@ template <int NC> __device__ __forceinline__ void tm_ld(float *v, uint32_t addr)
                        "=r"(u[k + 10]), "=r"(u[k + 11]), "=r"(u[k + 12]), "=r"(u[k + 13]),
                        "=r"(u[k + 14]), "=r"(u[k + 15])
                      : "r"(addr + k));
+    if (NC == 8)
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
+                       "=r"(u[6]), "=r"(u[7]) : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 template <int NC> __device__ __forceinline__ void tm_st(const float *v, uint32_t addr)
 {
     const uint32_t *u = reinterpret_cast<const uint32_t *>(v);
 #pragma unroll
-    for (int k = 0; k < NC; k += 16)
+    for (int k = 0; k + 16 <= NC; k += 16)
         asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
                      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                      ::"r"(addr + k), "r"(u[k]), "r"(u[k + 1]), "r"(u[k + 2]), "r"(u[k + 3]), "r"(u[k + 4]),
                        "r"(u[k + 5]), "r"(u[k + 6]), "r"(u[k + 7]), "r"(u[k + 8]), "r"(u[k + 9]),
                        "r"(u[k + 10]), "r"(u[k + 11]), "r"(u[k + 12]), "r"(u[k + 13]),
                        "r"(u[k + 14]), "r"(u[k + 15]) : "memory");
+    if (NC == 8)
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+                     ::"r"(addr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
+                       "r"(u[6]), "r"(u[7]) : "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
@@ -588,9 +611,10 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
  * l % NC. */
 template <int NC> __device__ __forceinline__ float lane_sums(float *v, int lane)
 {
-    if (NC == 16) {
 #pragma unroll
-        for (int i = 0; i < NC; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], 16);
+    for (int o = 16; o >= NC; o >>= 1) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
     }
 #pragma unroll
     for (int o = NC / 2; o > 0; o >>= 1) {
@@ -633,9 +657,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         for (int i = 0; i < Cfg::pairs; i++) { mbar_init(&c.pair_full[i], 1); mbar_init(&c.pair_empty[i], 1); }
         mbar_init(&c.rope_full, 1);
         mbar_init(&c.rope_empty, 1);
-        mbar_init(&c.q_full, 256);
+        mbar_init(&c.q_full, kTcSoft / 32);
         mbar_init(&c.s_full, 1);
-        mbar_init(&c.p_ready, 256);
+        mbar_init(&c.p_ready, kTcSoft / 32);
         mbar_init(&c.o_done, 1);
         mbar_init(&c.drain, 1);
         c.dead = 0;
@@ -648,8 +672,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;            /* O | S^T */
-    Seg g;
     if (any && warp == 0) {
+        Seg g;
         /* ---- loads: a lane a box of box_rows keys ---- */
         int it = 0;                                           /* pairs issued            */
         int ur = 0;                                           /* rope chunks issued      */
@@ -698,6 +722,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     } else if (any && warp == 1) {
         /* ---- products: one lane ---- */
         if (elect()) {
+            Seg g;
             constexpr uint32_t fmt = kF16 ? 0u : 1u;
             constexpr uint32_t id_s = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(N >> 3) << 17) | (8u << 24);
             constexpr uint32_t id_o = id_s | (1u << 15) | (1u << 16);
@@ -764,20 +789,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         __syncwarp();
     } else if (any && warp >= 2) {
         /* ---- softmax ---- */
-        const int st = tid - 64, half = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = half * NC;
+        constexpr float kNone = -1e30f;                       /* no reference yet            */
+        const int st = tid - 64, quarter = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = quarter * NC;
         const uint32_t tm_lane = (uint32_t)(quad * 32) << 16;
         const float scale2 = d.scale * 1.4426950408889634f;
-        float *mine = c.col[warp - 2];
-        int unit = 0, it = 0, segs = 0;
-        while (walk_next(p, w, g)) {
+        float(*mine)[16] = c.col[warp - 2];
+        float(*sx)[16] = c.mx[quarter];
+        int unit = 0, segs = 0, slot0 = 0, par0 = 0;
+        if (st == 0) c.walk = w;
+        const Seg &g = c.seg;
+        for (;;) {
+            bar_named(5, kTcSoft);                            /* the last segment is read    */
+            if (st == 0) {
+                Walk v = c.walk;
+                Seg n;
+                c.more = walk_next(p, v, n);
+                c.walk = v;
+                c.seg = n;
+            }
+            bar_named(5, kTcSoft);
+            if (!c.more) break;
             const bool whole = g.first && g.last;
             const int slot = part_slot(g);
-            float l[NC];
-            float ref = -INFINITY;                            /* of column c0 + lane        */
+            float l[NC], ref[NC];                             /* ref less the fp16 bias      */
 #pragma unroll
-            for (int i = 0; i < NC; i++) l[i] = 0.0f;
+            for (int i = 0; i < NC; i++) { l[i] = 0.0f; ref[i] = kNone; }
             /* the tile's rows: where they are, once */
-            bar_named(3, 256);                                /* the last segment's are read */
             if (st < N) {
                 const int at = g.row0 + st, tok = at / H, h = at - tok * H;
                 const bool in = st < g.rows;
@@ -785,14 +822,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * d.q_head_stride : -1;
                 c.ooff[st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
             }
-            bar_named(3, 256);
+            bar_named(5, kTcSoft);
             if (g.k0 < g.k1) {
                 /* the query tile: swizzled 128-byte rows, zeros past its rows and columns;
-                 * 32 rows by a chunk's eight 16-byte units at a time */
-                const int D = d.kl + d.rope, u = st & 7;
-#pragma unroll
-                for (int rb = 0; rb < N; rb += 32) {
-                    const int row = rb + (st >> 3);
+                 * a row's eight 16-byte units of a chunk to eight threads */
+                const int D = d.kl + d.rope, u = st & 7, row = st >> 3;
+                if (row < N) {
                     const long long off = c.qoff[row];
                     const T *src = static_cast<const T *>(d.q) + off + u * 8;
                     unsigned char *dst = sm + Cfg::off_q + row * 128 + ((u ^ (row & 7)) << 4);
@@ -806,53 +841,51 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         if (k < nchunk) *reinterpret_cast<uint4 *>(dst + k * N * 128) = v[k];
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                mbar_arrive(&c.q_full);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.q_full);
             }
-            for (int kt = g.k0; kt < g.k1; kt++, unit++, it += npair) {
-                const int key = kt * kTcKeys + key_row;
+            for (int kt = g.k0; kt < g.k1; kt++, unit++) {
                 const bool tail = kt * kTcKeys + kTcKeys > g.q.ctx || kt * kTcKeys + kTcKeys > g.vis;
                 float x[NC];
                 tc_wait(c, &c.s_full, unit & 1, p.err);
                 tc_fence_after();
                 tm_ld<NC>(x, tm_s + tm_lane + c0);
-#pragma unroll
-                for (int i = 0; i < NC; i++) x[i] *= scale2;
+                uint32_t seen = 0xffffffffu;                  /* columns that see this key   */
+                bool bad = false;
                 if (tail) {
                     /* rows past the request's are zeros to the second product, and so is
                      * a new row that holds a NaN or an infinity: who sees it gets NaN
-                     * weights, who does not is not touched */
-                    for (int j = 0; j < npair; j++)
-                        tc_wait(c, &c.pair_full[(it + j) % Cfg::pairs], ((it + j) / Cfg::pairs) & 1, p.err);
-                    if (half == 0) c.nan_row[key_row] = 0;
-                    bar_named(3, 256);
-                    if (key >= g.q.ctx && key < g.vis) {
-                        bool bad = false;
-                        for (int j = half; j < npair; j += 2) {
-                            const unsigned char *b = sm + ((it + j) % Cfg::pairs) * kPairBytes + key_row * 128;
-                            for (int u = 0; u < 16; u++) {
-                                const uint4 v = *reinterpret_cast<const uint4 *>(
-                                    b + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4));
-                                const uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u;
-                                bad |= __vcmpeq2(v.x & e, e) || __vcmpeq2(v.y & e, e) || __vcmpeq2(v.z & e, e) ||
-                                       __vcmpeq2(v.w & e, e);
-                            }
+                     * weights, who does not is not touched. A quarter takes a pair. */
+                    const int key = kt * kTcKeys + key_row;
+                    int sl = slot0 + quarter, pr = par0;
+                    if (sl >= Cfg::pairs) { sl -= Cfg::pairs; pr ^= 1; }
+                    unsigned char *mem = sm + sl * kPairBytes + key_row * 128;
+                    if (quarter < npair) tc_wait(c, &c.pair_full[sl], pr, p.err);
+                    if (quarter == 0) c.nan_row[key_row] = 0;
+                    bar_named(5, kTcSoft);
+                    if (quarter < npair && key >= g.q.ctx && key < g.vis) {
+                        bool found = false;
+                        for (int u = 0; u < 16; u++) {
+                            const uint4 v = *reinterpret_cast<const uint4 *>(
+                                mem + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4));
+                            const uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u;
+                            found |= __vcmpeq2(v.x & e, e) || __vcmpeq2(v.y & e, e) || __vcmpeq2(v.z & e, e) ||
+                                     __vcmpeq2(v.w & e, e);
                         }
-                        if (bad) c.nan_row[key_row] = 1;
+                        if (found) c.nan_row[key_row] = 1;
                     }
-                    bar_named(3, 256);
-                    const bool bad = c.nan_row[key_row];
-                    if (bad || key >= g.vis) {
-                        for (int j = half; j < npair; j += 2) {
-                            unsigned char *b = sm + ((it + j) % Cfg::pairs) * kPairBytes + key_row * 128;
-                            for (int u = 0; u < 16; u++)
-                                *reinterpret_cast<uint4 *>(b + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4)) =
-                                    make_uint4(0, 0, 0, 0);
-                        }
+                    bar_named(5, kTcSoft);
+                    bad = c.nan_row[key_row];
+                    if (quarter < npair && (bad || key >= g.vis)) {
+                        for (int u = 0; u < 16; u++)
+                            *reinterpret_cast<uint4 *>(mem + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4)) =
+                                make_uint4(0, 0, 0, 0);
                     }
                     const int nj = key - g.q.ctx;             /* its place among the new rows */
                     const bool in = key < g.vis;
                     int last = -1;
                     bool see = false;
+                    seen = 0;
 #pragma unroll
                     for (int i = 0; i < NC; i++) {
                         const int tok = c.tok[c0 + i];
@@ -860,49 +893,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                             last = tok;
                             see = in && (nj < 0 || (tok < g.q.n && sees(p, g.q, tok, nj)));
                         }
-                        if (!see) x[i] = -INFINITY;
-                        else if (bad) x[i] = __int_as_float(0x7fc00000);
+                        if (see) seen |= 1u << i;
+                        if (bad) x[i] = __int_as_float(0x7fc00000);
                     }
                 }
-                /* the columns' maxima over the tile's 128 keys */
-                float mx = -INFINITY;
+                float y[NC], top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < NC; i++) {
-                    const float m = warp_max(x[i]);
-                    if (lane == i) mx = m;
+                for (int i = 0; i < NC; i++) y[i] = fmaf(x[i], scale2, -ref[i]);
+                if (tail) {
+#pragma unroll
+                    for (int i = 0; i < NC; i++)
+                        if (!(seen >> i & 1)) y[i] = -INFINITY;
                 }
-                float (*sx)[32] = c.mx[unit & 1][half];
-                if (lane < NC) sx[quad][lane] = mx;
-                bar_named(1 + half, 128);
-                const int lc = lane % NC;
-                mx = fmaxf(fmaxf(sx[0][lc], sx[1][lc]), fmaxf(sx[2][lc], sx[3][lc]));
-                const bool grow = mx > ref + kLazy;           /* also at the first finite one */
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float a = grow ? (ref == -INFINITY ? 0.0f : ex2(ref - mx)) : 1.0f;
-                    if (grow) ref = mx;
-                    __syncwarp();
-                    if (lane < NC) mine[lane] = a;
-                    __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < NC; i++) l[i] *= mine[i];
+                for (int i = 0; i < NC; i++) top = fmaxf(top, y[i]);
+                if (bar_any(1 + quarter, top > kBias + kLazy)) {
+                    float mx = -INFINITY, r = kNone;          /* of column c0 + lane % NC     */
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        const float m = warp_max(seen >> i & 1 ? x[i] * scale2 : -INFINITY);
+                        if (lane % NC == i) { mx = m; r = ref[i]; }
+                    }
+                    if (lane < NC) sx[quad][lane] = mx;
+                    bar_named(1 + quarter, 128);
+                    mx = fmaxf(fmaxf(sx[0][lane % NC], sx[1][lane % NC]), fmaxf(sx[2][lane % NC], sx[3][lane % NC]));
+                    float a = 1.0f;
+                    if (mx > r + (kBias + kLazy)) {
+                        a = ex2(r - (mx - kBias));
+                        r = mx - kBias;
+                    }
+                    if (lane < NC) { mine[0][lane] = a; mine[1][lane] = r; }
+                    bar_named(1 + quarter, 128);              /* and sx is read              */
+#pragma unroll
+                    for (int i = 0; i < NC; i++) {
+                        l[i] *= mine[0][i];
+                        ref[i] = mine[1][i];
+                        y[i] = seen >> i & 1 ? fmaf(x[i], scale2, -ref[i]) : -INFINITY;
+                    }
                     if (kt > g.k0) {
                         /* the products before are done: S's commit followed them */
+#pragma unroll 1
                         for (int j = 0; j < npair; j++) {
                             float o[NC];
                             tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
 #pragma unroll
-                            for (int i = 0; i < NC; i++) o[i] *= mine[i];
+                            for (int i = 0; i < NC; i++) o[i] *= mine[0][i];
                             tm_st<NC>(o, tmem + tm_lane + j * N + c0);
                         }
                     }
+                    __syncwarp();
                 }
-                __syncwarp();
-                if (lane < NC) mine[lane] = (ref == -INFINITY ? 0.0f : ref) - kBias;
-                __syncwarp();
                 uint32_t pk[NC / 2];
 #pragma unroll
                 for (int i = 0; i < NC; i += 2) {
-                    const float e0 = ex2(x[i] - mine[i]), e1 = ex2(x[i + 1] - mine[i + 1]);
+                    const float e0 = ex2(y[i]), e1 = ex2(y[i + 1]);
                     l[i] += e0;
                     l[i + 1] += e1;
                     pk[i / 2] = pack2<T>(e0, e1);
@@ -915,20 +959,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         make_uint4(pk[4 * u], pk[4 * u + 1], pk[4 * u + 2], pk[4 * u + 3]);
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 tc_fence_before();
-                mbar_arrive(&c.p_ready);
+                __syncwarp();                                 /* an arrival a warp: they are serial */
+                if (lane == 0) mbar_arrive(&c.p_ready);
+                slot0 += npair;
+                if (slot0 >= Cfg::pairs) { slot0 -= Cfg::pairs; par0 ^= 1; }
             }
             /* ---- the segment's result ---- */
-            float sum = lane_sums<NC>(l, lane);               /* of column lane % NC         */
-            float (*sx)[32] = c.mx[unit & 1][half];
-            if (lane < NC) sx[quad][lane] = sum;
-            bar_named(1 + half, 128);
             const int lc = lane % NC;
+            float m = kNone;
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+                if (lc == i) m = ref[i];
+            float sum = lane_sums<NC>(l, lane);               /* of column c0 + lc           */
+            if (lane < NC) sx[quad][lane] = sum;
+            bar_named(1 + quarter, 128);
             sum = (sx[0][lc] + sx[1][lc]) + (sx[2][lc] + sx[3][lc]);
-            bar_named(1 + half, 128);                         /* read before it is reused    */
-            const float m = (ref == -INFINITY ? 0.0f : ref) - kBias;
-            __syncwarp();
-            if (lane < NC) mine[lane] = sum == 0.0f ? 0.0f : 1.0f / sum;
-            __syncwarp();
+            if (lane < NC) mine[0][lane] = sum == 0.0f ? 0.0f : 1.0f / sum;
+            bar_named(1 + quarter, 128);                      /* sx is read                  */
             const int row = c0 + lane;
             if (quad == 0 && lane < NC && row < g.rows) {
                 if (whole) {
@@ -957,7 +1004,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         T *dst = static_cast<T *>(d.o) + cd;
 #pragma unroll
                         for (int i = 0; i < NC; i++)
-                            if (i < nc) dst[c.ooff[c0 + i]] = from_f<T>(some && mine[i] != 0.0f ? o[i] * mine[i] : 0.0f);
+                            if (i < nc)
+                                dst[c.ooff[c0 + i]] = from_f<T>(some && mine[0][i] != 0.0f ? o[i] * mine[0][i] : 0.0f);
                     } else {
                         float *dst = p.part + ((size_t)slot * N + c0) * d.kl + cd;
 #pragma unroll
