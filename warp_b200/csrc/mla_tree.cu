@@ -48,53 +48,57 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
  * tile's keys come in tiles of KT. unit_prefix(i) is the number of units
  * before its tile i. In a chain of several tiles an early tile sees fewer
  * keys; its units are counted by a bound with a closed prefix sum,
- *   floor(sum_{j<i} (ctx + 1 + (j+1) NT/heads) / KT) + i,
- * which is at least the key tiles it sees and at most about one more (a unit
- * past them is empty). */
+ *   floor(sum_{j<i} (ctx + 1 + (j+1) NT/heads) / KT) + i
+ * (NT/heads in 2^-16, rounded up), which is at least the key tiles it sees
+ * and at most about one more (a unit past them is empty). Units are 32 bits
+ * wide: the host refuses calls whose sizes could pass that. At a kernel's
+ * start every instruction is a cold fetch, so this is kept short: the one
+ * thread that finds the CTA's first tile hands it to the others. */
 struct Req {
     int r, q0, n, ctx, kv, nt;       /* kv: rows seen at most, 0: nothing        */
-    int bad;
 };
 
 struct Shape {
     waste_cuda_mla_tree_desc d;
     int NT, KT, kt_log;              /* KT = 1 << kt_log                         */
+    unsigned int step;               /* NT / (2 heads) in 2^-16, rounded up       */
     unsigned int *err;
-    float *part;                     /* [2 * grid][NT][kl] partial sums          */
+    float *part;                     /* [2 * grid][NT][part_ld] partial sums      */
     float *stat;                     /* [2 * grid][NT][2] their maxima and sums  */
     int4 *meta;                      /* [grid] the tile that starts to be split there */
+    int part_ld;                     /* kl in whole float4s                       */
 };
-
-/* 64-bit quotients cost a few hundred cycles, and most here fit 32 bits */
-__device__ __forceinline__ unsigned long long div_u(unsigned long long a, unsigned long long b)
-{
-    return ((a | b) >> 32) ? a / b : (unsigned long long)((unsigned)a / (unsigned)b);
-}
 
 __device__ __forceinline__ Req req_at(const Shape &p, int r)
 {
     const waste_cuda_mla_tree_desc &d = p.d;
     Req q;
+    const int a = d.q_indptr[r], b = d.q_indptr[r + 1], kv = d.kv_len[r];
     q.r = r;
-    q.q0 = min(max(d.q_indptr[r], 0), d.T);
-    q.n = min(max(d.q_indptr[r + 1], q.q0), d.T) - q.q0;
-    const long long cap = (long long)d.max_blocks * d.page;
-    int kv = d.kv_len[r];
-    q.bad = kv > cap;
-    if (q.bad) kv = (int)cap;
-    q.kv = kv < q.n ? 0 : kv;
+    q.q0 = min(max(a, 0), d.T);
+    q.n = min(max(b, q.q0), d.T) - q.q0;
+    q.kv = min(kv, d.max_blocks * d.page);           /* longer: reported at the start */
+    q.kv = q.kv < q.n ? 0 : q.kv;
     q.ctx = q.kv - (q.kv ? q.n : 0);
     q.nt = (int)(((unsigned)q.n * (unsigned)d.heads + p.NT - 1u) / (unsigned)p.NT);
     return q;
 }
 
-__device__ __forceinline__ long long unit_prefix(const Shape &p, const Req &q, int i)
+__device__ __forceinline__ int unit_prefix(const Shape &p, const Req &q, int i)
 {
     if (!p.d.mask && q.nt > 1 && q.kv) {
-        const unsigned H2 = 2u * p.d.heads;
-        return (long long)(div_u(H2 * i * (q.ctx + 1ull) + (unsigned long long)p.NT * i * (i + 1ull), H2) >> p.kt_log) + i;
+        const unsigned long long k = (unsigned long long)i * (q.ctx + 1u);
+        return (int)((k + ((unsigned long long)i * (i + 1u) * p.step >> 16)) >> p.kt_log) + i;
     }
-    return (long long)i * max(1, (q.kv + p.KT - 1) >> p.kt_log);
+    return i * max(1, (q.kv + p.KT - 1) >> p.kt_log);
+}
+
+/* A CTA's place in the units: CTA c of G has [c * all / G, (c+1) * all / G)
+ * up to rounding; with fewer units than CTAs, the first CTAs have one each. */
+__device__ __forceinline__ int cta_of_unit(int u, int all)
+{
+    const int G = min((int)gridDim.x, all), per = all / G, rem = all - per * G, lim = rem * (per + 1);
+    return u < lim ? u / (per + 1) : rem + (u - lim) / per;
 }
 
 /* One CTA's share of one query tile: key tiles [k0, k1). */
@@ -102,101 +106,98 @@ struct Seg {
     Req q;
     int k0, k1;
     int vis;                         /* keys the tile's last row sees             */
-    bool first, last;                /* the tile's units all before / behind are here */
+    bool first, last;                /* the tile's first / last units are here    */
     int row0, rows;                  /* rows of the request                       */
-    long long tile_u0, tile_u1;      /* the tile's units, global                  */
+    int tile_u1;                     /* behind the tile's last unit               */
 };
 
 struct Walk {
-    long long u, u1;                 /* next unit, end                            */
-    long long base, tile_u0;         /* first unit of the request, of the tile    */
-    int r, tile;
+    int u, u1;                       /* next unit, end                            */
+    int tile, tile_u0;               /* the next tile, its first unit             */
     Req q;
+    int all;                         /* units of all CTAs                         */
 };
 
-/* All threads: the CTA's range of units and where it starts. `red` holds 67
- * long longs of shared memory. Returns false when the range is empty. */
-__device__ bool walk_begin(const Shape &p, Walk &w, long long *red, long long &total)
+struct WalkSmem {
+    int sum[32];                     /* units of a warp's requests                */
+    Walk w;
+};
+
+/* All threads (kWarps warps): the CTA's range of units and where it starts,
+ * in s.w; u == u1 where it has none. */
+template <int kWarps> __device__ __forceinline__ void walk_begin(const Shape &p, WalkSmem &s)
 {
-    const int nt = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, nw = nt >> 5;
-    const int per = (p.d.B + nt - 1) / nt, r0 = tid * per;
-    long long sum = 0;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int per = (p.d.B + kWarps * 32 - 1) / (kWarps * 32), r0 = tid * per;
+    int sum = 0;
     for (int k = 0; k < per && r0 + k < p.d.B; k++) {
         const Req q = req_at(p, r0 + k);
-        if (q.bad && blockIdx.x == 0) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+        if (blockIdx.x == 0 && p.d.kv_len[r0 + k] > p.d.max_blocks * p.d.page)
+            atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
         sum += unit_prefix(p, q, q.nt);
     }
-    long long inc = sum;
+    int at = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long a = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += a;
+        const int a = __shfl_up_sync(0xffffffffu, at, o);
+        if (lane >= o) at += a;
     }
-    if (lane == 31) red[warp] = inc;
+    if (lane == 31) s.sum[warp] = at;
     __syncthreads();
-    long long at = inc - sum, all = 0;
-#pragma unroll
-    for (int k = 0; k < 18; k++) {
-        const long long v = k < nw ? red[k] : 0;
-        if (k < warp) at += v;
-        all += v;
+    int v = lane < kWarps ? s.sum[lane] : 0;
+    const int all = __reduce_add_sync(0xffffffffu, v);
+    v = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+    at += v - sum;
+    const int G = min((int)gridDim.x, all), c = blockIdx.x;
+    int u = 0, u1 = 0;
+    if (c < G) {
+        const int each = all / G, rem = all - each * G;
+        u = c * each + min(c, rem);
+        u1 = u + each + (c < rem);
     }
-    total = all;
-    /* with fewer units than CTAs, the first CTAs take one each */
-    const long long G = max(1ll, min((long long)gridDim.x, all)), c = blockIdx.x;
-    w.u = c < G ? (long long)div_u(c * all, G) : all;
-    w.u1 = c < G ? (long long)div_u((c + 1) * all, G) : all;
-    if (sum > 0 && at <= w.u && w.u < at + sum) {
-        for (int k = 0; k < per && r0 + k < p.d.B; k++) {
+    if (tid == 0 && u == u1) s.w.u = s.w.u1 = 0;
+    if (u < u1 && at <= u && u < at + sum) {
+        for (int k = 0; k < per; k++) {
             const Req q = req_at(p, r0 + k);
-            const long long n = unit_prefix(p, q, q.nt);
-            if (w.u < at + n) {
+            const int n = unit_prefix(p, q, q.nt);
+            if (u < at + n) {
                 int lo = 0, hi = q.nt;
                 while (hi - lo > 1) {
                     const int mid = (lo + hi) >> 1;
-                    if (at + unit_prefix(p, q, mid) <= w.u) lo = mid; else hi = mid;
+                    if (at + unit_prefix(p, q, mid) <= u) lo = mid; else hi = mid;
                 }
-                red[64] = r0 + k;
-                red[65] = at;
-                red[66] = lo;
+                s.w = { u, u1, lo, at + unit_prefix(p, q, lo), q, all };
                 break;
             }
             at += n;
         }
     }
     __syncthreads();
-    if (w.u >= w.u1) return false;
-    w.r = (int)red[64];
-    w.base = red[65];
-    w.tile = (int)red[66];
-    w.q = req_at(p, w.r);
-    w.tile_u0 = w.base + unit_prefix(p, w.q, w.tile);
-    return true;
 }
 
 __device__ __forceinline__ bool walk_next(const Shape &p, Walk &w, Seg &s)
 {
     if (w.u >= w.u1) return false;
+    int base = w.tile_u0 - unit_prefix(p, w.q, w.tile);
     while (w.tile == w.q.nt) {
-        w.base = w.tile_u0;
-        w.q = req_at(p, ++w.r);
+        base = w.tile_u0;
+        w.q = req_at(p, w.q.r + 1);
         w.tile = 0;
     }
-    const int lo = w.tile++;
-    const int H = p.d.heads;
+    const int H = p.d.heads, u0 = w.tile_u0;
     s.q = w.q;
-    s.tile_u0 = w.tile_u0;
-    s.tile_u1 = w.tile_u0 = w.base + unit_prefix(p, w.q, lo + 1);
-    const long long end = min(s.tile_u1, w.u1);
-    s.first = w.u == s.tile_u0;
+    s.tile_u1 = w.tile_u0 = base + unit_prefix(p, w.q, w.tile + 1);
+    const int end = min(s.tile_u1, w.u1);
+    s.first = w.u == u0;
     s.last = end == s.tile_u1;
-    s.row0 = lo * p.NT;
+    s.row0 = w.tile * p.NT;
     s.rows = min(p.NT, w.q.n * H - s.row0);
     s.vis = p.d.mask || !w.q.kv ? w.q.kv : min(w.q.kv, w.q.ctx + (s.row0 + s.rows - 1) / H + 1);
     const int kt = (s.vis + p.KT - 1) >> p.kt_log;
-    s.k0 = (int)min((long long)kt, w.u - s.tile_u0);
-    s.k1 = (int)min((long long)kt, end - s.tile_u0);
+    s.k0 = min(kt, w.u - u0);
+    s.k1 = min(kt, end - u0);
     w.u = end;
+    w.tile++;
     return true;
 }
 
@@ -214,12 +215,10 @@ __device__ __forceinline__ int part_slot(const Seg &s) { return 2 * blockIdx.x +
 
 /* The CTA that holds a tile's first units names the tile for the combine:
  * {first row in tokens * heads, rows, last CTA, 1}. */
-__device__ __forceinline__ void note_split(const Shape &p, const Seg &s, long long total)
+__device__ __forceinline__ void note_split(const Shape &p, const Seg &s, int all)
 {
-    if (s.first && !s.last) {
-        const long long G = min((long long)gridDim.x, total), c1 = (long long)div_u(s.tile_u1 * G - 1, total);
-        p.meta[blockIdx.x] = make_int4(s.q.q0 * p.d.heads + s.row0, s.rows, (int)c1, 1);
-    }
+    if (s.first && !s.last)
+        p.meta[blockIdx.x] = make_int4(s.q.q0 * p.d.heads + s.row0, s.rows, cta_of_unit(s.tile_u1 - 1, all), 1);
 }
 
 /* ---- any type, size, stride and page ---------------------------------------
@@ -240,7 +239,7 @@ struct GenSmem {
     float p[kGenKeys][kGenRows];     /* scores, then weights                      */
     float m[kGenRows], l[kGenRows], a[kGenRows];
     long long off[kGenKeys];         /* element offset of a key's row, -1: none   */
-    long long red[67];
+    WalkSmem walk;
 };
 
 template <typename T>
@@ -255,9 +254,8 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
     const T *cache = static_cast<const T *>(d.cache);
     wc_pdl::trigger();
     if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-    Walk w;
-    long long total;
-    if (!walk_begin(p, w, s.red, total)) return;
+    walk_begin<kGenThreads / 32>(p, s.walk);
+    Walk w = s.walk.w;
     Seg g;
     while (walk_next(p, w, g)) {
         const int rows = g.rows;
@@ -407,7 +405,7 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                                           (size_t)(at % H) * d.o_head_stride + j] =
                         from_f<T>(l == 0.0f ? 0.0f : acc[z][i] * inv);
                 else
-                    p.part[((size_t)slot * kGenRows + i) * kl + j] = acc[z][i];
+                    p.part[((size_t)slot * kGenRows + i) * p.part_ld + j] = acc[z][i];
             }
         }
         if (tid < rows) {
@@ -420,7 +418,7 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                 p.stat[((size_t)slot * kGenRows + tid) * 2 + 1] = l;
             }
         }
-        if (tid == 0) note_split(p, g, total);
+        if (tid == 0) note_split(p, g, w.all);
     }
 }
 
@@ -475,15 +473,14 @@ struct TcCtl {
     uint64_t rope_full, rope_empty, q_full, s_full, p_ready, o_done, drain;
     uint32_t tmem;
     volatile int dead;
-    long long red[67];
+    WalkSmem walk;
     float mx[4][4][16];              /* [quarter][quadrant][column]                  */
     float col[16][2][16];            /* a warp's broadcast of values a column         */
-    long long qoff[64], ooff[64];    /* a tile row's elements in q (-1: no row) and o */
+    long long qoff[64], ooff[2][64]; /* a tile row's elements in q (-1: no row) and o */
     int tok[64];                     /* its token in the request                     */
     unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
-    Walk walk;                       /* the softmax warps' schedule, and their segment */
-    Seg seg;
-    int more;
+    Seg seg[2];                      /* the softmax warps' segment and the next       */
+    int more[2];
 };
 
 __device__ __forceinline__ bool tc_wait(TcCtl &c, uint64_t *bar, uint32_t parity, unsigned int *err)
@@ -665,12 +662,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         c.dead = 0;
         mbar_fence_init();
     }
-    Walk w;
-    long long total;
-    const bool any = walk_begin(p, w, c.red, total);
     tc_fence_before();
-    __syncthreads();
+    walk_begin<kTcThreads / 32>(p, c.walk);
     tc_fence_after();
+    Walk w = c.walk.w;
+    const bool any = w.u < w.u1;
     const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;            /* O | S^T */
     if (any && warp == 0) {
         Seg g;
@@ -796,54 +792,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         float(*mine)[16] = c.col[warp - 2];
         float(*sx)[16] = c.mx[quarter];
         int unit = 0, segs = 0, slot0 = 0, par0 = 0;
-        if (st == 0) c.walk = w;
-        const Seg &g = c.seg;
-        for (;;) {
-            bar_named(5, kTcSoft);                            /* the last segment is read    */
-            if (st == 0) {
-                Walk v = c.walk;
-                Seg n;
-                c.more = walk_next(p, v, n);
-                c.walk = v;
-                c.seg = n;
-            }
-            bar_named(5, kTcSoft);
-            if (!c.more) break;
-            const bool whole = g.first && g.last;
-            const int slot = part_slot(g);
-            float l[NC], ref[NC];                             /* ref less the fp16 bias      */
-#pragma unroll
-            for (int i = 0; i < NC; i++) { l[i] = 0.0f; ref[i] = kNone; }
-            /* the tile's rows: where they are, once */
+        /* tables of segment i's rows, and its query tile: swizzled 128-byte rows,
+         * zeros past its rows and columns, a row's eight 16-byte units of a chunk
+         * to eight threads */
+        auto tables = [&](int i) {
+            const Seg &g = c.seg[i];
             if (st < N) {
                 const int at = g.row0 + st, tok = at / H, h = at - tok * H;
                 const bool in = st < g.rows;
                 c.tok[st] = in ? tok : 0x3fffffff;
                 c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * d.q_head_stride : -1;
-                c.ooff[st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
+                c.ooff[i][st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
             }
-            bar_named(5, kTcSoft);
-            if (g.k0 < g.k1) {
-                /* the query tile: swizzled 128-byte rows, zeros past its rows and columns;
-                 * a row's eight 16-byte units of a chunk to eight threads */
-                const int D = d.kl + d.rope, u = st & 7, row = st >> 3;
-                if (row < N) {
-                    const long long off = c.qoff[row];
-                    const T *src = static_cast<const T *>(d.q) + off + u * 8;
-                    unsigned char *dst = sm + Cfg::off_q + row * 128 + ((u ^ (row & 7)) << 4);
-                    uint4 v[9];
+        };
+        auto queries = [&](int i) {
+            if (c.seg[i].k0 == c.seg[i].k1) return;
+            const int D = d.kl + d.rope, u = st & 7, row = st >> 3;
+            if (row < N) {
+                const long long off = c.qoff[row];
+                const T *src = static_cast<const T *>(d.q) + off + u * 8;
+                unsigned char *dst = sm + Cfg::off_q + row * 128 + ((u ^ (row & 7)) << 4);
+                uint4 v[9];
 #pragma unroll
-                    for (int k = 0; k < 9; k++)
-                        v[k] = off >= 0 && k < nchunk && k * 64 + u * 8 < D
-                                   ? __ldg(reinterpret_cast<const uint4 *>(src + k * 64)) : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < 9; k++)
+                    v[k] = off >= 0 && k < nchunk && k * 64 + u * 8 < D
+                               ? __ldg(reinterpret_cast<const uint4 *>(src + k * 64)) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-                    for (int k = 0; k < 9; k++)
-                        if (k < nchunk) *reinterpret_cast<uint4 *>(dst + k * N * 128) = v[k];
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&c.q_full);
+                for (int k = 0; k < 9; k++)
+                    if (k < nchunk) *reinterpret_cast<uint4 *>(dst + k * N * 128) = v[k];
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.q_full);
+        };
+        auto next = [&](int i) {                              /* one thread                  */
+            Walk v = c.walk.w;
+            Seg n;
+            c.more[i] = walk_next(p, v, n);
+            c.walk.w = v;
+            c.seg[i] = n;
+        };
+        bar_named(5, kTcSoft);                                /* every role has the start    */
+        if (st == 0) next(0);
+        bar_named(5, kTcSoft);
+        tables(0);
+        bar_named(5, kTcSoft);
+        queries(0);
+        for (int cur = 0;; cur ^= 1) {
+            const Seg &g = c.seg[cur];
+            if (st == 0) next(cur ^ 1);                       /* while the first tile loads  */
+            const bool whole = g.first && g.last;
+            const int slot = part_slot(g);
+            float l[NC], ref[NC];                             /* ref less the fp16 bias      */
+#pragma unroll
+            for (int i = 0; i < NC; i++) { l[i] = 0.0f; ref[i] = kNone; }
             for (int kt = g.k0; kt < g.k1; kt++, unit++) {
                 const bool tail = kt * kTcKeys + kTcKeys > g.q.ctx || kt * kTcKeys + kTcKeys > g.vis;
                 float x[NC];
@@ -964,6 +966,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 slot0 += npair;
                 if (slot0 >= Cfg::pairs) { slot0 -= Cfg::pairs; par0 ^= 1; }
             }
+            /* the next segment's queries first: its products run under what follows */
+            bar_named(5, kTcSoft);
+            const bool more = c.more[cur ^ 1];
+            if (more) {
+                tables(cur ^ 1);
+                bar_named(5, kTcSoft);
+                queries(cur ^ 1);
+            }
             /* ---- the segment's result ---- */
             const int lc = lane % NC;
             float m = kNone;
@@ -1005,17 +1015,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
 #pragma unroll
                         for (int i = 0; i < NC; i++)
                             if (i < nc)
-                                dst[c.ooff[c0 + i]] = from_f<T>(some && mine[0][i] != 0.0f ? o[i] * mine[0][i] : 0.0f);
+                                dst[c.ooff[cur][c0 + i]] = from_f<T>(some && mine[0][i] != 0.0f ? o[i] * mine[0][i] : 0.0f);
                     } else {
-                        float *dst = p.part + ((size_t)slot * N + c0) * d.kl + cd;
+                        float *dst = p.part + (slot * N + c0) * p.part_ld + cd;
 #pragma unroll
                         for (int i = 0; i < NC; i++)
-                            if (i < nc) dst[(size_t)i * d.kl] = o[i];
+                            if (i < nc) dst[i * p.part_ld] = o[i];
                     }
                 }
             }
             tc_fence_before();
-            if (st == 0) note_split(p, g, total);
+            if (st == 0) note_split(p, g, w.all);
+            if (!more) break;
         }
     }
     __syncthreads();
@@ -1026,55 +1037,85 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
 
 /* ---- split tiles joined ------------------------------------------------------
  * grid (CTAs of the attention, rows of a tile): the tile whose first units
- * CTA c held, one row. o = sum_s e^(m_s - M) o_s / sum_s e^(m_s - M) l_s over
- * its segments in key order. Bound by reading the partial sums, from L2.
- * LOG2: the maxima are in units of log2. */
+ * CTA c held, one row. o = sum_s w_s o_s / sum_s w_s l_s, w_s = e^(m_s - M),
+ * over its segments in key order. Bound by reading the partial sums from
+ * L2, so the weights of all segments are found first, a thread each, and a
+ * thread then has kCombDeep segments' loads in flight. LOG2: the maxima are
+ * in units of log2. */
 constexpr int kCombThreads = 128;
+constexpr int kCombDeep = 8;
+constexpr int kCombMax = 256;        /* CTAs of the attention at most             */
 
 template <typename T, int LOG2>
 __global__ void __launch_bounds__(kCombThreads) mla_combine_kernel(const __grid_constant__ Shape p)
 {
+    __shared__ float sw[kCombMax], red[kCombThreads / 32], sums[kCombMax];
     wc_pdl::wait();
     const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
     const int4 t = p.meta[c];
     if (!t.w || row >= t.y) return;
     const waste_cuda_mla_tree_desc &d = p.d;
-    const int kl = d.kl;
+    const int kl = d.kl, n = t.z - c + 1;
     const float ln2 = 0.693147180559945f;
+    auto at_slot = [&](int k) { return (k == 0 ? 2 * c + 1 : 2 * (c + k)) * p.NT + row; };
     float M = -INFINITY;
-    for (int k = c; k <= t.z; k++) {
-        const int slot = k == c ? 2 * c + 1 : 2 * k;
-        M = fmaxf(M, p.stat[((size_t)slot * p.NT + row) * 2]);
+    for (int k = tid; k < n; k += kCombThreads) {
+        const float2 ml = *reinterpret_cast<const float2 *>(p.stat + (size_t)at_slot(k) * 2);
+        sw[k] = ml.x;
+        sums[k] = ml.y;
+        M = fmaxf(M, ml.x);
     }
-    const float ref = M == -INFINITY ? 0.0f : M;
-    float acc[kMaxKl / kCombThreads] = {}, L = 0.0f;
-    for (int k = c; k <= t.z; k++) {
-        const int slot = k == c ? 2 * c + 1 : 2 * k;
-        const float m = p.stat[((size_t)slot * p.NT + row) * 2], l = p.stat[((size_t)slot * p.NT + row) * 2 + 1];
-        if (l == 0.0f) continue;                     /* saw nothing: its sums are not set */
-        const float e = LOG2 ? exp2f(m - ref) : expf(m - ref);
-        L = fmaf(e, l, L);
-        const float *o = p.part + ((size_t)slot * p.NT + row) * kl;
 #pragma unroll
-        for (int j = 0; j < kMaxKl / kCombThreads; j++)
-            if (tid + j * kCombThreads < kl) acc[j] = fmaf(e, o[tid + j * kCombThreads], acc[j]);
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    if ((tid & 31) == 0) red[tid >> 5] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    for (int k = tid; k < n; k += kCombThreads) {
+        /* a segment that saw nothing weighs nothing: its sums are not set */
+        const float m = sw[k] - (M == -INFINITY ? 0.0f : M);
+        sw[k] = sums[k] == 0.0f ? 0.0f : (LOG2 ? exp2f(m) : expf(m));
+    }
+    __syncthreads();
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float L = 0.0f;
+    const float4 *part = reinterpret_cast<const float4 *>(p.part);
+    const int ld = p.part_ld / 4;
+    const bool in = tid < ld;
+    for (int k0 = 0; k0 < n; k0 += kCombDeep) {
+        float4 v[kCombDeep];
+#pragma unroll
+        for (int u = 0; u < kCombDeep; u++)
+            v[u] = in && k0 + u < n && sums[k0 + u] != 0.0f ? part[(size_t)at_slot(k0 + u) * ld + tid]
+                                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int u = 0; u < kCombDeep; u++) {
+            if (k0 + u >= n) break;
+            const float e = sw[k0 + u];
+            L = fmaf(e, sums[k0 + u], L);
+            acc.x = fmaf(e, v[u].x, acc.x);
+            acc.y = fmaf(e, v[u].y, acc.y);
+            acc.z = fmaf(e, v[u].z, acc.z);
+            acc.w = fmaf(e, v[u].w, acc.w);
+        }
     }
     const int at = t.x + row, tok = at / d.heads, h = at - tok * d.heads;
-    T *o = static_cast<T *>(d.o) + (size_t)tok * d.o_token_stride + (size_t)h * d.o_head_stride;
+    T *o = static_cast<T *>(d.o) + (size_t)tok * d.o_token_stride + (size_t)h * d.o_head_stride + tid * 4;
+    const float vals[4] = { acc.x, acc.y, acc.z, acc.w };
 #pragma unroll
-    for (int j = 0; j < kMaxKl / kCombThreads; j++)
-        if (tid + j * kCombThreads < kl)
-            o[tid + j * kCombThreads] = from_f<T>(L == 0.0f ? 0.0f : acc[j] / L);
+    for (int j = 0; j < 4; j++)
+        if (tid * 4 + j < kl) o[j] = from_f<T>(L == 0.0f ? 0.0f : vals[j] / L);
     if (tid == 0 && d.lse)
         d.lse[at] = L == 0.0f ? -INFINITY : (LOG2 ? (M + log2f(L)) * ln2 : M + logf(L));
 }
 
-/* the workspace: partial sums | their statistics | the split tiles */
+/* the workspace: partial sums | their statistics | the split tiles (each in whole 16 bytes) */
 void carve(Shape *p, int grid)
 {
     char *w = static_cast<char *>(p->d.ws);
+    p->step = (unsigned)(((unsigned long long)p->NT * 65536 + 2ull * p->d.heads - 1) / (2ull * p->d.heads));
+    p->part_ld = (p->d.kl + 3) & ~3;
     p->part = reinterpret_cast<float *>(w);
-    w += (size_t)2 * grid * p->NT * p->d.kl * sizeof(float);
+    w += (size_t)2 * grid * p->NT * p->part_ld * sizeof(float);
     p->stat = reinterpret_cast<float *>(w);
     w += (size_t)2 * grid * p->NT * 2 * sizeof(float);
     p->meta = reinterpret_cast<int4 *>(w);
@@ -1150,7 +1191,7 @@ int wc_mla_tree_box(const waste_cuda_mla_tree_desc *d)
 
 size_t wc_mla_tree_ws_bytes(int kl, int sms)
 {
-    return (size_t)2 * sms * kTileMax * (kl + 2) * sizeof(float) + (size_t)sms * sizeof(int4);
+    return (size_t)2 * sms * kTileMax * (((kl + 3) & ~3) + 2) * sizeof(float) + (size_t)sms * sizeof(int4);
 }
 
 int wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *map, int box_rows,
