@@ -223,129 +223,166 @@ __device__ __forceinline__ void note_split(const Shape &p, const Seg &s, int all
 
 /* ---- any type, size, stride and page ---------------------------------------
  * fp32 arithmetic throughout. A CTA of 256 threads takes 32 query rows by
- * tiles of 64 keys. Scores: a warp takes 8 keys, 4 at a time, their values
- * strided over the lanes in registers, against 8 query rows at a time from
- * shared memory; the 32 sums of a batch are reduced across the lanes
- * together (31 shuffles), one (row, key) to a lane. Products: a thread owns
- * two of the kl columns for all 32 rows (64 sums in registers), the weights
- * broadcast from shared memory, the cache rows read again through L2. The
- * FMA rate bounds it from a few rows on. */
+ * tiles of 32 keys, both as fp32 rows in shared memory, rows 16 bytes past a
+ * multiple of 128 apart so that float4 loads of successive rows meet no bank
+ * twice. Scores: two groups of four warps take half of the columns each, a
+ * thread 4 rows by 2 keys (6 loads of 16 bytes for 32 FMAs), and the halves
+ * are added. Products: a thread owns two of the kl columns for all rows, the
+ * weights broadcast (10 loads' worth of shared memory for 64 FMAs a key).
+ * So the FMA rate bounds it: 32 x 32 rows of 512 + 64 are 8.7 k cycles of
+ * it. Where rows are fp32 and 16-byte aligned the next tile's are copied
+ * asynchronously meanwhile, if two tiles fit. */
 constexpr int kGenThreads = 256;
 constexpr int kGenRows = 32;
-constexpr int kGenKeys = 64;
-constexpr int kGenJ = (kMaxKl + kMaxRope) / 32;
+constexpr int kGenKeys = 32;
 
-struct GenSmem {
-    float p[kGenKeys][kGenRows];     /* scores, then weights                      */
+struct alignas(16) GenSmem {
+    float p[kGenKeys][kGenRows];     /* scores (key, row), then weights           */
+    float h[kGenKeys][kGenRows];     /* the second half's scores                  */
     float m[kGenRows], l[kGenRows], a[kGenRows];
-    long long off[kGenKeys];         /* element offset of a key's row, -1: none   */
+    int tok[kGenRows];               /* a row's token in the request              */
+    int bad[kGenKeys];               /* a new row that holds no finite number     */
     WalkSmem walk;
 };
 
+static_assert(sizeof(GenSmem) % 16 == 0, "rows behind it are read as float4");
+
+__host__ __device__ constexpr int gen_ld(int D) { return ((D + 31) & ~31) + 4; }
+
 template <typename T>
-__global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_constant__ Shape p)
+__global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_constant__ Shape p, int bufs,
+                                                                 int async)
 {
     extern __shared__ __align__(16) unsigned char smg[];
     GenSmem &s = *reinterpret_cast<GenSmem *>(smg);
-    float *qs = reinterpret_cast<float *>(smg + sizeof(GenSmem));    /* [32][D] */
     const waste_cuda_mla_tree_desc &d = p.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int H = d.heads, kl = d.kl, D = d.kl + d.rope, nj = (D + 31) / 32;
+    const int H = d.heads, kl = d.kl, D = d.kl + d.rope, ld = gen_ld(D), nv = (D + 3) / 4;
+    float *qs = reinterpret_cast<float *>(smg + sizeof(GenSmem));    /* [32][ld]       */
+    float *ks = qs + kGenRows * ld;                                  /* [bufs][32][ld] */
     const T *cache = static_cast<const T *>(d.cache);
     wc_pdl::trigger();
     if (tid == 0) p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
+    /* the columns between D and the next float4 stay zero */
+    for (int i = tid; i < (1 + bufs) * kGenRows * 4; i += kGenThreads)
+        if (D + (i & 3) < nv * 4) qs[(i >> 2) * ld + D + (i & 3)] = 0.0f;
     walk_begin<kGenThreads / 32>(p, s.walk);
     Walk w = s.walk.w;
     Seg g;
+    /* tile kt of the segment into buffer `buf`: 8 threads a key, rows past the
+     * last seen one zero */
+    auto fetch = [&](const Seg &g, int kt, int buf) {
+        const int k = tid >> 3, sub = tid & 7, key = kt * kGenKeys + k;
+        float *dst = ks + (buf * kGenKeys + k) * ld;
+        bool in = key < g.vis;
+        const T *src = cache;
+        if (in) {
+            const int b = key / d.page, id = d.block_table[(size_t)g.q.r * d.max_blocks + b];
+            in = id >= 0 && id < d.n_blocks;
+            if (!in && sub == 0) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+            if (in) src += ((long long)id * d.page + (key - b * d.page)) * (long long)d.row_stride;
+        }
+        if (async) {
+            for (int i = sub; i < nv; i += 8)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                             ::"r"(smem_u32(dst + i * 4)), "l"(src + i * 4), "r"(in ? 16 : 0) : "memory");
+        } else {
+#pragma unroll 8
+            for (int i = sub; i < D; i += 8) dst[i] = in ? to_f(src[i]) : 0.0f;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
     while (walk_next(p, w, g)) {
         const int rows = g.rows;
         __syncthreads();
-        for (int i = tid; i < kGenRows * D; i += kGenThreads) {
-            const int row = i / D, j = i - row * D, at = g.row0 + row;
-            qs[i] = row < rows ? to_f(static_cast<const T *>(d.q)[(size_t)(g.q.q0 + at / H) * d.q_token_stride +
-                                                                 (size_t)(at % H) * d.q_head_stride + j])
-                               : 0.0f;
+        if (g.k0 < g.k1) fetch(g, g.k0, 0);
+        if (tid < kGenRows) {
+            s.m[tid] = -INFINITY;
+            s.l[tid] = 0.0f;
+            s.tok[tid] = (g.row0 + tid) / H;
         }
-        if (tid < kGenRows) { s.m[tid] = -INFINITY; s.l[tid] = 0.0f; }
+        __syncthreads();
+        for (int i = tid >> 3; i < kGenRows; i += kGenThreads / 8) {
+            const int tok = s.tok[i], h = g.row0 + i - tok * H;
+            const T *src = static_cast<const T *>(d.q) + (size_t)(g.q.q0 + tok) * d.q_token_stride +
+                           (size_t)h * d.q_head_stride;
+#pragma unroll 8
+            for (int j = tid & 7; j < D; j += 8) qs[i * ld + j] = i < rows ? to_f(src[j]) : 0.0f;
+        }
         float acc[2][kGenRows];
 #pragma unroll
         for (int i = 0; i < kGenRows; i++) acc[0][i] = acc[1][i] = 0.0f;
         for (int kt = g.k0; kt < g.k1; kt++) {
-            const int k0 = kt * kGenKeys, nk = min(kGenKeys, g.vis - k0);
-            const bool tail = k0 + nk > g.q.ctx;
+            const int k0 = kt * kGenKeys, buf = bufs == 2 ? (kt - g.k0) & 1 : 0;
+            const bool tail = k0 + kGenKeys > g.q.ctx || k0 + kGenKeys > g.vis;
+            float *kb = ks + buf * kGenKeys * ld;
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();
-            if (tid < nk) {
-                const int key = k0 + tid, b = key / d.page;
-                const int id = d.block_table[(size_t)g.q.r * d.max_blocks + b];
-                const bool ok = id >= 0 && id < d.n_blocks;
-                if (!ok) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
-                s.off[tid] = ok ? ((long long)id * d.page + (key - b * d.page)) * (long long)d.row_stride : -1;
+            if (bufs == 2 && kt + 1 < g.k1) fetch(g, kt + 1, buf ^ 1);
+            {
+                const int half = warp >> 2, t4 = tid & 127, rg = t4 & 7, kg = t4 >> 3;   /* rows rg + 8i, keys kg + 16j */
+                float sum[4][2] = {};
+                if (rg < rows) {
+                    const float *qp = qs + rg * ld, *kp = kb + kg * ld;
+#pragma unroll 4
+                    for (int v = half; v < nv; v += 2) {
+                        float4 q[4], k[2];
+#pragma unroll
+                        for (int i = 0; i < 4; i++) q[i] = *reinterpret_cast<const float4 *>(qp + i * 8 * ld + v * 4);
+#pragma unroll
+                        for (int j = 0; j < 2; j++) k[j] = *reinterpret_cast<const float4 *>(kp + j * 16 * ld + v * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+#pragma unroll
+                            for (int j = 0; j < 2; j++) {
+                                sum[i][j] = fmaf(q[i].x, k[j].x, sum[i][j]);
+                                sum[i][j] = fmaf(q[i].y, k[j].y, sum[i][j]);
+                                sum[i][j] = fmaf(q[i].z, k[j].z, sum[i][j]);
+                                sum[i][j] = fmaf(q[i].w, k[j].w, sum[i][j]);
+                            }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 2; j++) (half ? s.h : s.p)[kg + 16 * j][rg + 8 * i] = sum[i][j];
+            }
+            if (tail) {
+                /* a new row that holds a NaN or an infinity is zeros to the products;
+                 * who sees it gets NaN weights, who does not is not touched */
+                const int k = tid >> 3, key = k0 + k;
+                float *row = kb + k * ld;
+                bool bad = false;
+                if (key >= g.q.ctx && key < g.vis)
+                    for (int i = tid & 7; i < kl; i += 8) bad |= !isfinite(row[i]);
+                bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 24)) & 0xff;
+                if ((tid & 7) == 0) s.bad[k] = bad;
+                __syncthreads();                              /* the scores have read it     */
+                if (bad)
+                    for (int i = tid & 7; i < kl; i += 8) row[i] = 0.0f;
             }
             __syncthreads();
-#pragma unroll 1
-            for (int kb = warp * 8; kb < warp * 8 + 8; kb += 4) {
-                float c[4][kGenJ];
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const long long off = kb + k < nk ? s.off[kb + k] : -1;
-#pragma unroll
-                    for (int j = 0; j < kGenJ; j++)
-                        c[k][j] = j < nj && off >= 0 && lane + 32 * j < D ? to_f(cache[off + lane + 32 * j]) : 0.0f;
-                }
-#pragma unroll 1
-                for (int rb = 0; rb < rows; rb += 8) {
-                    float sum[32];                       /* [8 rows][4 keys] */
-#pragma unroll
-                    for (int i = 0; i < 32; i++) sum[i] = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < kGenJ; j++) {
-                        if (j >= nj) break;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const float q = lane + 32 * j < D ? qs[(rb + i) * D + lane + 32 * j] : 0.0f;
-#pragma unroll
-                            for (int k = 0; k < 4; k++) sum[i * 4 + k] = fmaf(q, c[k][j], sum[i * 4 + k]);
-                        }
-                    }
-                    /* halve the sums a lane holds at each step: lane l ends
-                     * with sum l */
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) {
-                        const bool up = lane & o;
-#pragma unroll
-                        for (int i = 0; i < o; i++) {
-                            const float give = up ? sum[i] : sum[i + o];
-                            const float got = __shfl_xor_sync(0xffffffffu, give, o);
-                            sum[i] = (up ? sum[i + o] : sum[i]) + got;
-                        }
-                    }
-                    const int row = rb + (lane >> 2), k = kb + (lane & 3), key = k0 + k;
-                    const int tok = (g.row0 + row) / H;
-                    bool see = row < rows && k < nk && s.off[k] >= 0;
-                    if (see && key >= g.q.ctx) see = sees(p, g.q, tok, key - g.q.ctx);
-                    s.p[k][row] = see ? sum[0] * d.scale : -INFINITY;
-                }
-            }
-            __syncthreads();
-            /* softmax of 4 rows a warp; two keys a lane */
+            /* softmax: a key a lane, 4 rows a warp */
 #pragma unroll
             for (int i = 0; i < kGenRows / 8; i++) {
-                const int row = warp * (kGenRows / 8) + i;
+                const int row = warp + 8 * i, key = k0 + lane;
                 if (row >= rows) break;
-                const float x0 = lane < nk ? s.p[lane][row] : -INFINITY;
-                const float x1 = lane + 32 < nk ? s.p[lane + 32][row] : -INFINITY;
-                float mx = fmaxf(x0, x1);
+                float x = (s.p[lane][row] + s.h[lane][row]) * d.scale;
+                if (tail) {
+                    const bool see = key < g.vis && (key < g.q.ctx || sees(p, g.q, s.tok[row], key - g.q.ctx));
+                    if (!see) x = -INFINITY;
+                    else if (s.bad[lane]) x = __int_as_float(0x7fc00000);
+                }
+                float mx = x;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                 const float m0 = s.m[row], m1 = fmaxf(m0, mx), ref = m1 == -INFINITY ? 0.0f : m1;
                 /* a masked key weighs exactly nothing; a NaN score stays one */
-                const float e0 = x0 == -INFINITY ? 0.0f : expf(x0 - ref);
-                const float e1 = x1 == -INFINITY ? 0.0f : expf(x1 - ref);
-                float sum = e0 + e1;
+                const float e = x == -INFINITY ? 0.0f : expf(x - ref);
+                float sum = e;
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                s.p[lane][row] = e0;
-                s.p[lane + 32][row] = e1;
+                s.p[lane][row] = e;
                 __syncwarp();
                 if (lane == 0) {
                     const float a = m0 == -INFINITY ? 0.0f : expf(m0 - ref);
@@ -355,57 +392,53 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                 }
             }
             __syncthreads();
+            const int c0 = 2 * tid;
 #pragma unroll
-            for (int i = 0; i < kGenRows; i++) {
-                const float a = i < rows ? s.a[i] : 0.0f;
-                acc[0][i] *= a;
-                acc[1][i] *= a;
+            for (int i = 0; i < kGenRows / 4; i++) {
+                if (4 * i >= rows) break;
+                const float4 a = *reinterpret_cast<const float4 *>(s.a + 4 * i);
+                const float aa[4] = { a.x, a.y, a.z, a.w };
+#pragma unroll
+                for (int z = 0; z < 4; z++) { acc[0][4 * i + z] *= aa[z]; acc[1][4 * i + z] *= aa[z]; }
             }
-            const bool c0 = tid < kl, c1 = tid + kGenThreads < kl;
+            if (c0 < kl) {
 #pragma unroll 4
-            for (int k = 0; k < nk; k++) {
-                const long long off = s.off[k];
-                const float v0 = c0 && off >= 0 ? to_f(cache[off + tid]) : 0.0f;
-                const float v1 = c1 && off >= 0 ? to_f(cache[off + tid + kGenThreads]) : 0.0f;
-                const float4 *pk = reinterpret_cast<const float4 *>(s.p[k]);
-                /* a row that does not see a new key is not to meet its
-                 * values: they may be no numbers */
-                const bool finite = isfinite(v0) && isfinite(v1);
+                for (int k = 0; k < kGenKeys; k++) {
+                    const float2 v = *reinterpret_cast<const float2 *>(kb + k * ld + c0);
+                    const float4 *pk = reinterpret_cast<const float4 *>(s.p[k]);
 #pragma unroll
-                for (int i = 0; i < kGenRows / 4; i++) {
-                    const float4 e = pk[i];
-                    const float ee[4] = { e.x, e.y, e.z, e.w };
+                    for (int i = 0; i < kGenRows / 4; i++) {
+                        if (4 * i >= rows) break;
+                        const float4 e = pk[i];
+                        const float ee[4] = { e.x, e.y, e.z, e.w };
 #pragma unroll
-                    for (int z = 0; z < 4; z++) {
-                        if (finite || !tail) {
-                            acc[0][4 * i + z] = fmaf(ee[z], v0, acc[0][4 * i + z]);
-                            acc[1][4 * i + z] = fmaf(ee[z], v1, acc[1][4 * i + z]);
-                        } else if (ee[z] != 0.0f) {
-                            acc[0][4 * i + z] += ee[z] * v0;
-                            acc[1][4 * i + z] += ee[z] * v1;
+                        for (int z = 0; z < 4; z++) {
+                            acc[0][4 * i + z] = fmaf(ee[z], v.x, acc[0][4 * i + z]);
+                            acc[1][4 * i + z] = fmaf(ee[z], v.y, acc[1][4 * i + z]);
                         }
                     }
                 }
             }
+            if (bufs == 1 && kt + 1 < g.k1) {
+                __syncthreads();
+                fetch(g, kt + 1, 0);
+            }
         }
         __syncthreads();
         const bool whole = g.first && g.last;
-        const int slot = part_slot(g);
+        const int slot = part_slot(g), c0 = 2 * tid;
 #pragma unroll
         for (int i = 0; i < kGenRows; i++) {
             if (i >= rows) break;
-            const int at = g.row0 + i;
             const float l = s.l[i], inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-            for (int z = 0; z < 2; z++) {
-                const int j = tid + z * kGenThreads;
-                if (j >= kl) continue;
-                if (whole)
-                    static_cast<T *>(d.o)[(size_t)(g.q.q0 + at / H) * d.o_token_stride +
-                                          (size_t)(at % H) * d.o_head_stride + j] =
-                        from_f<T>(l == 0.0f ? 0.0f : acc[z][i] * inv);
-                else
-                    p.part[((size_t)slot * kGenRows + i) * p.part_ld + j] = acc[z][i];
+            if (whole) {
+                const int tok = s.tok[i], h = g.row0 + i - tok * H;
+                T *o = static_cast<T *>(d.o) + (size_t)(g.q.q0 + tok) * d.o_token_stride + (size_t)h * d.o_head_stride;
+                if (c0 < kl) o[c0] = from_f<T>(l == 0.0f ? 0.0f : acc[0][i] * inv);
+                if (c0 + 1 < kl) o[c0 + 1] = from_f<T>(l == 0.0f ? 0.0f : acc[1][i] * inv);
+            } else {
+                float *o = p.part + ((size_t)slot * kGenRows + i) * p.part_ld;
+                if (c0 < p.part_ld) *reinterpret_cast<float2 *>(o + c0) = make_float2(acc[0][i], acc[1][i]);
             }
         }
         if (tid < rows) {
@@ -1128,13 +1161,17 @@ cudaError_t gen_launch(Shape &p, int sms, cudaStream_t s)
 {
     p.NT = kGenRows;
     p.KT = kGenKeys;
-    p.kt_log = 6;
+    p.kt_log = 5;
     carve(&p, sms);
-    const size_t smem = sizeof(GenSmem) + (size_t)kGenRows * (p.d.kl + p.d.rope) * sizeof(float);
+    const int D = p.d.kl + p.d.rope, ld = gen_ld(D);
+    const int async = sizeof(T) == 4 && D % 4 == 0 && p.d.row_stride % 4 == 0 && ((uintptr_t)p.d.cache & 15) == 0;
+    size_t smem = sizeof(GenSmem) + (size_t)3 * kGenRows * ld * sizeof(float);
+    const int bufs = smem <= 227 * 1024 ? 2 : 1;
+    if (bufs == 1) smem -= (size_t)kGenRows * ld * sizeof(float);
     cudaError_t e = cudaFuncSetAttribute(mla_gen_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
-    mla_gen_kernel<T><<<sms, kGenThreads, smem, s>>>(p);
+    mla_gen_kernel<T><<<sms, kGenThreads, smem, s>>>(p, bufs, async);
     wc_count_launches(1);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     e = wc_pdl::launch(mla_combine_kernel<T, 0>, dim3(sms, p.NT), dim3(kCombThreads), 0, s, true, p);

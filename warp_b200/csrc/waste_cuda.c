@@ -3389,9 +3389,9 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("mla_tree_attn_dev"))) goto out;
-    /* the kernels count (32 rows, 64 keys) units in 32 bits */
+    /* the kernels count (32 rows, 32 keys) units in 32 bits */
     if ((int64_t)d->T * d->heads > 1 << 25 ||
-        ((int64_t)d->T * d->heads / 32 + d->B + 1) * ((int64_t)d->page * d->max_blocks / 64 + 2) > INT32_MAX) {
+        ((int64_t)d->T * d->heads / 32 + d->B + 1) * ((int64_t)d->page * d->max_blocks / 32 + 2) > INT32_MAX) {
         rc = fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: %d tokens of %d heads over %d blocks of %d", d->T,
                   d->heads, d->max_blocks, d->page);
         goto out;
