@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             if (!in && sub == 0) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
             if (in) src += ((long long)id * d.page + (key - b * d.page)) * (long long)d.row_stride;
         }
-        if (async) {
+        if (async & 1) {
             for (int i = sub; i < nv; i += 8)
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
                              ::"r"(smem_u32(dst + i * 4)), "l"(src + i * 4), "r"(in ? 16 : 0) : "memory");
@@ -302,12 +302,19 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             s.tok[tid] = (g.row0 + tid) / H;
         }
         __syncthreads();
-        for (int i = tid >> 3; i < kGenRows; i += kGenThreads / 8) {
-            const int tok = s.tok[i], h = g.row0 + i - tok * H;
-            const T *src = static_cast<const T *>(d.q) + (size_t)(g.q.q0 + tok) * d.q_token_stride +
-                           (size_t)h * d.q_head_stride;
+        {
+            const int i = tid >> 3, tok = s.tok[i], h = g.row0 + i - tok * H;
+            const T *src = static_cast<const T *>(d.q);
+            if (i < rows) src += (size_t)(g.q.q0 + tok) * d.q_token_stride + (size_t)h * d.q_head_stride;
+            if (async & 2) {
+                for (int j = tid & 7; j < nv; j += 8)
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                 ::"r"(smem_u32(qs + i * ld + j * 4)), "l"(src + j * 4), "r"(i < rows ? 16 : 0) : "memory");
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            } else {
 #pragma unroll 8
-            for (int j = tid & 7; j < D; j += 8) qs[i * ld + j] = i < rows ? to_f(src[j]) : 0.0f;
+                for (int j = tid & 7; j < D; j += 8) qs[i * ld + j] = i < rows ? to_f(src[j]) : 0.0f;
+            }
         }
         float acc[2][kGenRows];
 #pragma unroll
@@ -508,9 +515,10 @@ struct TcCtl {
     volatile int dead;
     WalkSmem walk;
     float mx[4][4][16];              /* [quarter][quadrant][column]                  */
-    float col[16][2][16];            /* a warp's broadcast of values a column         */
+    float col[4][2][16];             /* [quarter] two values of each column           */
     long long qoff[64], ooff[2][64]; /* a tile row's elements in q (-1: no row) and o */
     int tok[64];                     /* its token in the request                     */
+    uint32_t krow[kTcKeys];          /* a key's row of the cache, without TMA         */
     unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
     Seg seg[2];                      /* the softmax warps' segment and the next       */
     int more[2];
@@ -659,7 +667,7 @@ template <int NC> __device__ __forceinline__ float lane_sums(float *v, int lane)
     return v[0];
 }
 
-template <typename T, int N>
+template <typename T, int N, bool TMA>
 __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_constant__ Shape p,
                                                                const __grid_constant__ CUtensorMap map,
                                                                int box_rows)
@@ -674,7 +682,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     TcCtl &c = *reinterpret_cast<TcCtl *>(sm + Cfg::off_ctl);
     const waste_cuda_mla_tree_desc &d = p.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int npair = d.kl / 128, nchunk = d.kl / 64 + (d.rope > 0), H = d.heads;
+    const int npair = (d.kl + 127) / 128, nchunk = d.kl / 64 + (d.rope > 0), H = d.heads;
+    const bool odd = d.kl & 64;                               /* the last pair is one chunk  */
 
     wc_pdl::trigger();
     if (warp == 1) {
@@ -684,8 +693,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     }
     if (tid == 0) {
         p.meta[blockIdx.x] = make_int4(0, 0, 0, 0);
-        for (int i = 0; i < Cfg::pairs; i++) { mbar_init(&c.pair_full[i], 1); mbar_init(&c.pair_empty[i], 1); }
-        mbar_init(&c.rope_full, 1);
+        for (int i = 0; i < Cfg::pairs; i++) { mbar_init(&c.pair_full[i], TMA ? 1 : 32); mbar_init(&c.pair_empty[i], 1); }
+        mbar_init(&c.rope_full, TMA ? 1 : 32);
         mbar_init(&c.rope_empty, 1);
         mbar_init(&c.q_full, kTcSoft / 32);
         mbar_init(&c.s_full, 1);
@@ -703,50 +712,114 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     const uint32_t tmem = c.tmem, tm_s = tmem + 4 * N;            /* O | S^T */
     if (any && warp == 0) {
         Seg g;
-        /* ---- loads: a lane a box of box_rows keys ---- */
-        int it = 0;                                           /* pairs issued            */
-        int ur = 0;                                           /* rope chunks issued      */
-        while (walk_next(p, w, g)) {
-            for (int kt = g.k0; kt < g.k1; kt++) {
-                const int k0 = kt * kTcKeys, nk = min(kTcKeys, g.vis - k0);
-                const int nbox = (nk + box_rows - 1) / box_rows;
-                int blk = 0, row = 0;
-                if (lane < nbox) {
-                    const int key = k0 + lane * box_rows, b = key / d.page;
-                    row = key - b * d.page;
-                    blk = d.block_table[(size_t)g.q.r * d.max_blocks + b];
-                    if (blk < 0 || blk >= d.n_blocks) {
-                        atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
-                        blk = (int)d.n_blocks;              /* reads zeros */
-                    }
-                }
-                const uint32_t chunk_tx = (uint32_t)(nbox * box_rows) * 128u;
-                for (int j = 0; j <= npair; j++) {
-                    const bool rope = j == npair;
-                    if (rope && d.rope == 0) continue;
-                    uint64_t *full = rope ? &c.rope_full : &c.pair_full[it % Cfg::pairs];
-                    uint64_t *empty = rope ? &c.rope_empty : &c.pair_empty[it % Cfg::pairs];
-                    const int use = rope ? ur : it / Cfg::pairs;
-                    bool ok = true;
-                    if (use > 0) ok = tc_wait(c, empty, (use - 1) & 1, p.err);
-                    ok = __all_sync(0xffffffffu, ok && !c.dead);
-                    if (!ok) continue;
-                    if (lane == 0) mbar_expect_tx(full, rope ? chunk_tx : 2 * chunk_tx);
-                    __syncwarp();
+        int it = 0, ur = 0;                                   /* pairs and rope chunks issued */
+        if (TMA) {
+            /* ---- loads: a lane a box of box_rows keys ---- */
+            while (walk_next(p, w, g)) {
+                for (int kt = g.k0; kt < g.k1; kt++) {
+                    const int k0 = kt * kTcKeys, nk = min(kTcKeys, g.vis - k0);
+                    const int nbox = (nk + box_rows - 1) / box_rows;
+                    int blk = 0, row = 0;
                     if (lane < nbox) {
-                        unsigned char *dst = sm + (rope ? Cfg::off_rope : (it % Cfg::pairs) * kPairBytes) +
-                                             lane * box_rows * 128;
-                        tma_load_3d(dst, &map, j * 128, row, blk, full);
-                        if (!rope) tma_load_3d(dst + kTcKeys * 128, &map, j * 128 + 64, row, blk, full);
+                        const int key = k0 + lane * box_rows, b = key / d.page;
+                        row = key - b * d.page;
+                        blk = d.block_table[(size_t)g.q.r * d.max_blocks + b];
+                        if (blk < 0 || blk >= d.n_blocks) {
+                            atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+                            blk = (int)d.n_blocks;            /* reads zeros                 */
+                        }
                     }
-                    if (rope) ur++; else it++;
+                    const uint32_t chunk_tx = (uint32_t)(nbox * box_rows) * 128u;
+                    for (int j = 0; j <= npair; j++) {
+                        const bool rope = j == npair, both = !rope && !(odd && j == npair - 1);
+                        if (rope && d.rope == 0) continue;
+                        uint64_t *full = rope ? &c.rope_full : &c.pair_full[it % Cfg::pairs];
+                        uint64_t *empty = rope ? &c.rope_empty : &c.pair_empty[it % Cfg::pairs];
+                        const int use = rope ? ur : it / Cfg::pairs;
+                        bool ok = true;
+                        if (use > 0) ok = tc_wait(c, empty, (use - 1) & 1, p.err);
+                        ok = __all_sync(0xffffffffu, ok && !c.dead);
+                        if (!ok) continue;
+                        if (lane == 0) mbar_expect_tx(full, both ? 2 * chunk_tx : chunk_tx);
+                        __syncwarp();
+                        if (lane < nbox) {
+                            unsigned char *dst = sm + (rope ? Cfg::off_rope : (it % Cfg::pairs) * kPairBytes) +
+                                                 lane * box_rows * 128;
+                            tma_load_3d(dst, &map, rope ? d.kl : j * 128, row, blk, full);
+                            if (both) tma_load_3d(dst + kTcKeys * 128, &map, j * 128 + 64, row, blk, full);
+                        }
+                        if (rope) ur++; else it++;
+                    }
                 }
             }
-        }
-        if (c.dead) {                                         /* what is in flight lands */
-            for (int i = 0; i < Cfg::pairs; i++)
-                if (it > i) mbar_wait(&c.pair_full[i], ((it - 1 - i) / Cfg::pairs) & 1);
-            if (ur > 0) mbar_wait(&c.rope_full, (ur - 1) & 1);
+            if (c.dead) {                                     /* what is in flight lands     */
+                for (int i = 0; i < Cfg::pairs; i++)
+                    if (it > i) mbar_wait(&c.pair_full[i], ((it - 1 - i) / Cfg::pairs) & 1);
+                if (ur > 0) mbar_wait(&c.rope_full, (ur - 1) & 1);
+            }
+        } else {
+            /* ---- loads of other pages: 16 bytes a lane, 8 lanes a row's chunk. What was
+             * issued is handed over before any wait for room, and at the end ---- */
+            uint64_t *pend[kMaxPairs + 1];
+            int npend = 0;
+            auto flush = [&]() {
+                asm volatile("cp.async.wait_all;" ::: "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i <= kMaxPairs; i++)
+                    if (i < npend) mbar_arrive(pend[i]);
+                npend = 0;
+            };
+            constexpr uint32_t kNoRow = 0xffffffffu;
+            const T *cache = static_cast<const T *>(d.cache);
+            const int u = lane & 7;
+            while (walk_next(p, w, g)) {
+                for (int kt = g.k0; kt < g.k1; kt++) {
+                    const int k0 = kt * kTcKeys;
+                    __syncwarp();
+                    for (int i = lane; i < kTcKeys; i += 32) {
+                        const int key = k0 + i, b = key / d.page;
+                        uint32_t row = kNoRow;
+                        if (key < g.vis) {
+                            const int id = d.block_table[(size_t)g.q.r * d.max_blocks + b];
+                            if (id < 0 || id >= d.n_blocks) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+                            else row = (uint32_t)id * (uint32_t)d.page + (uint32_t)(key - b * d.page);
+                        }
+                        c.krow[i] = row;
+                    }
+                    __syncwarp();
+                    for (int j = 0; j <= npair; j++) {
+                        const bool rope = j == npair, both = !rope && !(odd && j == npair - 1);
+                        if (rope && d.rope == 0) continue;
+                        uint64_t *full = rope ? &c.rope_full : &c.pair_full[it % Cfg::pairs];
+                        uint64_t *empty = rope ? &c.rope_empty : &c.pair_empty[it % Cfg::pairs];
+                        const int use = rope ? ur : it / Cfg::pairs;
+                        bool ok = true;
+                        if (use > 0) {
+                            flush();
+                            ok = tc_wait(c, empty, (use - 1) & 1, p.err);
+                        }
+                        ok = __all_sync(0xffffffffu, ok && !c.dead);
+                        if (!ok) continue;
+                        const uint32_t dst = smem_u32(sm + (rope ? Cfg::off_rope : (it % Cfg::pairs) * kPairBytes));
+                        const int col = (rope ? d.kl : j * 128) + u * 8, end = rope ? d.kl + d.rope : d.kl;
+                        for (int r = lane >> 3; r < kTcKeys; r += 4) {
+                            const uint32_t row = c.krow[r];
+                            const bool in = row != kNoRow;
+                            const T *src = cache + (in ? (size_t)row * d.row_stride : 0) + (col < end ? col : 0);
+                            const uint32_t to = dst + r * 128 + ((u ^ (r & 7)) << 4);
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                         ::"r"(to), "l"(src), "r"(in && col < end ? 16 : 0) : "memory");
+                            if (both)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                                             ::"r"(to + kTcKeys * 128), "l"(src + 64), "r"(in ? 16 : 0) : "memory");
+                        }
+                        pend[npend++] = full;
+                        if (rope) ur++; else it++;
+                    }
+                }
+            }
+            flush();
         }
     } else if (any && warp == 1) {
         /* ---- products: one lane ---- */
@@ -774,16 +847,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         ok = tc_wait(c, &c.pair_full[slot], par, p.err);
                         if (!ok) break;
                         const uint32_t a = k_lo + slot * (kPairBytes / 16), b = q_lo + j * (2 * N * 128 / 16);
+                        const int steps = odd && j == npair - 1 ? 4 : 8;
 #pragma unroll
                         for (int k = 0; k < 8; k++)
-                            tc_mma<kHi, kHi>(tm_s, a + (k >> 2) * (kTcKeys * 128 / 16) + (k & 3) * 2,
+                            if (k < steps) tc_mma<kHi, kHi>(tm_s, a + (k >> 2) * (kTcKeys * 128 / 16) + (k & 3) * 2,
                                              b + (k >> 2) * (N * 128 / 16) + (k & 3) * 2, id_s, (j | k) != 0);
                         if (++slot == Cfg::pairs) { slot = 0; par ^= 1; }
                     }
                     if (d.rope > 0 && ok) {
                         ok = tc_wait(c, &c.rope_full, unit & 1, p.err);
                         if (!ok) break;
-                        const uint32_t b = q_lo + npair * (2 * N * 128 / 16);
+                        const uint32_t b = q_lo + (d.kl / 64) * (N * 128 / 16);
                         for (int k = 0; k < rope_steps; k++)
                             tc_mma<kHi, kHi>(tm_s, r_lo + k * 2, b + k * 2, id_s, 1u);
                     }
@@ -822,7 +896,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         const int st = tid - 64, quarter = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = quarter * NC;
         const uint32_t tm_lane = (uint32_t)(quad * 32) << 16;
         const float scale2 = d.scale * 1.4426950408889634f;
-        float(*mine)[16] = c.col[warp - 2];
+        float(*mine)[16] = c.col[quarter];                    /* the 4 warps write the same  */
         float(*sx)[16] = c.mx[quarter];
         int unit = 0, segs = 0, slot0 = 0, par0 = 0;
         /* tables of segment i's rows, and its query tile: swizzled 128-byte rows,
@@ -895,12 +969,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     int sl = slot0 + quarter, pr = par0;
                     if (sl >= Cfg::pairs) { sl -= Cfg::pairs; pr ^= 1; }
                     unsigned char *mem = sm + sl * kPairBytes + key_row * 128;
+                    const int units = odd && quarter == npair - 1 ? 8 : 16;
                     if (quarter < npair) tc_wait(c, &c.pair_full[sl], pr, p.err);
                     if (quarter == 0) c.nan_row[key_row] = 0;
                     bar_named(5, kTcSoft);
                     if (quarter < npair && key >= g.q.ctx && key < g.vis) {
                         bool found = false;
-                        for (int u = 0; u < 16; u++) {
+                        for (int u = 0; u < units; u++) {
                             const uint4 v = *reinterpret_cast<const uint4 *>(
                                 mem + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4));
                             const uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u;
@@ -912,7 +987,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     bar_named(5, kTcSoft);
                     bad = c.nan_row[key_row];
                     if (quarter < npair && (bad || key >= g.vis)) {
-                        for (int u = 0; u < 16; u++)
+                        for (int u = 0; u < units; u++)
                             *reinterpret_cast<uint4 *>(mem + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4)) =
                                 make_uint4(0, 0, 0, 0);
                     }
@@ -1043,6 +1118,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     float o[NC];
                     if (some) tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
                     const int cd = j * 128 + key_row;
+                    if (cd >= d.kl) continue;                 /* the last chunk has no pair   */
                     if (whole) {
                         T *dst = static_cast<T *>(d.o) + cd;
 #pragma unroll
@@ -1069,76 +1145,145 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
 }
 
 /* ---- split tiles joined ------------------------------------------------------
- * grid (CTAs of the attention, rows of a tile): the tile whose first units
- * CTA c held, one row. o = sum_s w_s o_s / sum_s w_s l_s, w_s = e^(m_s - M),
- * over its segments in key order. Bound by reading the partial sums from
- * L2, so the weights of all segments are found first, a thread each, and a
- * thread then has kCombDeep segments' loads in flight. LOG2: the maxima are
+ * o = sum_s w_s o_s / sum_s w_s l_s, w_s = e^(m_s - M), over a split tile's
+ * segments in key order. Bound by reading the partial sums from L2, so each
+ * thread has kCombDeep segments' loads in flight. The blocks (four an SM, all
+ * resident) share out the list of split tiles that the attention left: with
+ * few segments two rows at a time, 128 threads of float4s each; with many (a
+ * long row alone on the GPU) a quarter of a row's columns, a warp an eighth of
+ * the segments in turns, the warps' sums added in order. LOG2: the maxima are
  * in units of log2. */
-constexpr int kCombThreads = 128;
+constexpr int kCombThreads = 256;
 constexpr int kCombDeep = 8;
 constexpr int kCombMax = 256;        /* CTAs of the attention at most             */
 
 template <typename T, int LOG2>
-__global__ void __launch_bounds__(kCombThreads) mla_combine_kernel(const __grid_constant__ Shape p)
+__global__ void __launch_bounds__(kCombThreads, 4) mla_combine_kernel(const __grid_constant__ Shape p, int ctas)
 {
-    __shared__ float sw[kCombMax], red[kCombThreads / 32], sums[kCombMax];
+    __shared__ int4 meta[kCombMax];
+    __shared__ int start[kCombMax + 1];
+    __shared__ float sw[kCombMax], red[8], redl[8];
+    __shared__ __align__(16) float4 part_s[8][32];
     wc_pdl::wait();
-    const int c = blockIdx.x, row = blockIdx.y, tid = threadIdx.x;
-    const int4 t = p.meta[c];
-    if (!t.w || row >= t.y) return;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const waste_cuda_mla_tree_desc &d = p.d;
-    const int kl = d.kl, n = t.z - c + 1;
-    const float ln2 = 0.693147180559945f;
-    auto at_slot = [&](int k) { return (k == 0 ? 2 * c + 1 : 2 * (c + k)) * p.NT + row; };
-    float M = -INFINITY;
-    for (int k = tid; k < n; k += kCombThreads) {
-        const float2 ml = *reinterpret_cast<const float2 *>(p.stat + (size_t)at_slot(k) * 2);
-        sw[k] = ml.x;
-        sums[k] = ml.y;
-        M = fmaxf(M, ml.x);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    if ((tid & 31) == 0) red[tid >> 5] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    for (int k = tid; k < n; k += kCombThreads) {
-        /* a segment that saw nothing weighs nothing: its sums are not set */
-        const float m = sw[k] - (M == -INFINITY ? 0.0f : M);
-        sw[k] = sums[k] == 0.0f ? 0.0f : (LOG2 ? exp2f(m) : expf(m));
-    }
-    __syncthreads();
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float L = 0.0f;
+    const int kl = d.kl, ld = p.part_ld / 4;
     const float4 *part = reinterpret_cast<const float4 *>(p.part);
-    const int ld = p.part_ld / 4;
-    const bool in = tid < ld;
-    for (int k0 = 0; k0 < n; k0 += kCombDeep) {
-        float4 v[kCombDeep];
+    const float2 *stat = reinterpret_cast<const float2 *>(p.stat);
+    {
+        const int4 t = tid < ctas ? p.meta[tid] : make_int4(0, 0, 0, 0);
+        const int items = !t.w ? 0 : t.z - tid < kCombDeep ? (t.y + 1) / 2 : 4 * t.y;
+        int at = items;
 #pragma unroll
-        for (int u = 0; u < kCombDeep; u++)
-            v[u] = in && k0 + u < n && sums[k0 + u] != 0.0f ? part[(size_t)at_slot(k0 + u) * ld + tid]
-                                                             : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int u = 0; u < kCombDeep; u++) {
-            if (k0 + u >= n) break;
-            const float e = sw[k0 + u];
-            L = fmaf(e, sums[k0 + u], L);
-            acc.x = fmaf(e, v[u].x, acc.x);
-            acc.y = fmaf(e, v[u].y, acc.y);
-            acc.z = fmaf(e, v[u].z, acc.z);
-            acc.w = fmaf(e, v[u].w, acc.w);
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
         }
+        meta[tid] = t;
+        if (lane == 31) start[warp] = at;
+        __syncthreads();
+        int v = lane < 8 ? start[lane] : 0;
+        v = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
+        __syncthreads();
+        start[tid] = at + v - items;
+        if (tid == kCombMax - 1) start[kCombMax] = at + v;
+        __syncthreads();
     }
-    const int at = t.x + row, tok = at / d.heads, h = at - tok * d.heads;
-    T *o = static_cast<T *>(d.o) + (size_t)tok * d.o_token_stride + (size_t)h * d.o_head_stride + tid * 4;
-    const float vals[4] = { acc.x, acc.y, acc.z, acc.w };
+    const int items = start[kCombMax];
+    auto store = [&](int row, int col, float4 acc, float L, float M) {
+        const int tok = row / d.heads, h = row - tok * d.heads;
+        T *o = static_cast<T *>(d.o) + (size_t)tok * d.o_token_stride + (size_t)h * d.o_head_stride + col * 4;
+        const float vals[4] = { acc.x, acc.y, acc.z, acc.w };
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        if (tid * 4 + j < kl) o[j] = from_f<T>(L == 0.0f ? 0.0f : vals[j] / L);
-    if (tid == 0 && d.lse)
-        d.lse[at] = L == 0.0f ? -INFINITY : (LOG2 ? (M + log2f(L)) * ln2 : M + logf(L));
+        for (int j = 0; j < 4; j++)
+            if (col * 4 + j < kl) o[j] = from_f<T>(L == 0.0f ? 0.0f : vals[j] * inv);
+        if (col == 0 && d.lse)
+            d.lse[row] = L == 0.0f ? -INFINITY : (LOG2 ? (M + log2f(L)) * 0.693147180559945f : M + logf(L));
+    };
+    auto add = [](float4 &a, float e, float4 v) {
+        a.x = fmaf(e, v.x, a.x);
+        a.y = fmaf(e, v.y, a.y);
+        a.z = fmaf(e, v.z, a.z);
+        a.w = fmaf(e, v.w, a.w);
+    };
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        int c = 0;                                            /* the last with start <= item */
+#pragma unroll
+        for (int o = kCombMax / 2; o > 0; o >>= 1)
+            if (start[c + o] <= item) c += o;
+        const int4 t = meta[c];
+        const int n = t.z - c + 1, at = item - start[c];
+        auto slot = [&](int k, int row) { return (size_t)((k == 0 ? 2 * c + 1 : 2 * (c + k)) * p.NT + row); };
+        if (n <= kCombDeep) {
+            const int row = at * 2 + (tid >> 7), col = tid & 127;
+            if (row >= t.y) continue;
+            float2 ml[kCombDeep];
+            float4 v[kCombDeep];
+#pragma unroll
+            for (int u = 0; u < kCombDeep; u++) {
+                ml[u] = u < n ? stat[slot(u, row)] : make_float2(-INFINITY, 0.0f);
+                v[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (u < n && col < ld) v[u] = part[slot(u, row) * ld + col];
+            }
+            float M = -INFINITY, L = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kCombDeep; u++) M = fmaxf(M, ml[u].x);
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < kCombDeep; u++) {
+                /* a segment that saw nothing weighs nothing: its sums are not set */
+                if (ml[u].y == 0.0f) continue;
+                const float x = ml[u].x - (M == -INFINITY ? 0.0f : M), e = LOG2 ? exp2f(x) : expf(x);
+                L = fmaf(e, ml[u].y, L);
+                add(acc, e, v[u]);
+            }
+            store(t.x + row, col, acc, L, M);
+            continue;
+        }
+        const int row = at >> 2, col = (at & 3) * 32 + lane;
+        float2 ml = make_float2(-INFINITY, 0.0f);             /* segment tid's               */
+        if (tid < n) ml = stat[slot(tid, row)];
+        float M = ml.x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        if (lane == 0) red[warp] = M;
+        __syncthreads();
+        M = red[0];
+#pragma unroll
+        for (int k = 1; k < 8; k++) M = fmaxf(M, red[k]);
+        const float x = ml.x - (M == -INFINITY ? 0.0f : M);
+        const float e = ml.y == 0.0f ? 0.0f : (LOG2 ? exp2f(x) : expf(x));
+        sw[tid] = e;
+        float L = e * ml.y;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane == 0) redl[warp] = L;
+        __syncthreads();
+        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k0 = warp * kCombDeep; k0 < n; k0 += 8 * kCombDeep) {
+            float4 v[kCombDeep];
+#pragma unroll
+            for (int u = 0; u < kCombDeep; u++)
+                v[u] = col < ld && k0 + u < n && sw[k0 + u] != 0.0f ? part[slot(k0 + u, row) * ld + col]
+                                                                     : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int u = 0; u < kCombDeep; u++)
+                if (k0 + u < n) add(acc, sw[k0 + u], v[u]);
+        }
+        part_s[warp][lane] = acc;
+        __syncthreads();
+        if (warp == 0 && col < ld) {
+            L = redl[0];
+#pragma unroll
+            for (int k = 1; k < 8; k++) {
+                add(acc, 1.0f, part_s[k][lane]);
+                L += redl[k];
+            }
+            store(t.x + row, col, acc, L, M);
+        }
+        __syncthreads();
+    }
 }
 
 /* the workspace: partial sums | their statistics | the split tiles (each in whole 16 bytes) */
@@ -1164,7 +1309,12 @@ cudaError_t gen_launch(Shape &p, int sms, cudaStream_t s)
     p.kt_log = 5;
     carve(&p, sms);
     const int D = p.d.kl + p.d.rope, ld = gen_ld(D);
-    const int async = sizeof(T) == 4 && D % 4 == 0 && p.d.row_stride % 4 == 0 && ((uintptr_t)p.d.cache & 15) == 0;
+    /* bit 0: the cache's rows are copied asynchronously, bit 1: the queries' */
+    int async = 0;
+    if (sizeof(T) == 4 && D % 4 == 0) {
+        async |= p.d.row_stride % 4 == 0 && ((uintptr_t)p.d.cache & 15) == 0;
+        async |= p.d.q_token_stride % 4 == 0 && p.d.q_head_stride % 4 == 0 && ((uintptr_t)p.d.q & 15) == 0 ? 2 : 0;
+    }
     size_t smem = sizeof(GenSmem) + (size_t)3 * kGenRows * ld * sizeof(float);
     const int bufs = smem <= 227 * 1024 ? 2 : 1;
     if (bufs == 1) smem -= (size_t)kGenRows * ld * sizeof(float);
@@ -1174,12 +1324,12 @@ cudaError_t gen_launch(Shape &p, int sms, cudaStream_t s)
     mla_gen_kernel<T><<<sms, kGenThreads, smem, s>>>(p, bufs, async);
     wc_count_launches(1);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    e = wc_pdl::launch(mla_combine_kernel<T, 0>, dim3(sms, p.NT), dim3(kCombThreads), 0, s, true, p);
+    e = wc_pdl::launch(mla_combine_kernel<T, 0>, dim3(4 * sms), dim3(kCombThreads), 0, s, true, p, sms);
     wc_count_launches(1);
     return e;
 }
 
-template <typename T, int N>
+template <typename T, int N, bool TMA>
 cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, cudaStream_t s)
 {
     p.NT = N;
@@ -1188,13 +1338,13 @@ cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, c
     carve(&p, sms);
     const size_t smem = TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024;
     static_assert(TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024 <= 227 * 1024, "attention tile exceeds shared memory");
-    cudaError_t e = cudaFuncSetAttribute(mla_tc_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(mla_tc_kernel<T, N, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
-    mla_tc_kernel<T, N><<<sms, kTcThreads, smem, s>>>(p, map, box_rows);
+    mla_tc_kernel<T, N, TMA><<<sms, kTcThreads, smem, s>>>(p, map, box_rows);
     wc_count_launches(1);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    e = wc_pdl::launch(mla_combine_kernel<T, 1>, dim3(sms, N), dim3(kCombThreads), 0, s, true, p);
+    e = wc_pdl::launch(mla_combine_kernel<T, 1>, dim3(4 * sms), dim3(kCombThreads), 0, s, true, p, sms);
     wc_count_launches(1);
     return e;
 }
@@ -1202,8 +1352,10 @@ cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, c
 template <typename T>
 cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, cudaStream_t s)
 {
-    return (long long)p.d.T * p.d.heads <= 32ll * p.d.B ? tc_launch<T, 32>(p, map, box_rows, sms, s)
-                                                        : tc_launch<T, 64>(p, map, box_rows, sms, s);
+    const bool few = (long long)p.d.T * p.d.heads <= 32ll * p.d.B;
+    if (box_rows > 1)
+        return few ? tc_launch<T, 32, true>(p, map, box_rows, sms, s) : tc_launch<T, 64, true>(p, map, box_rows, sms, s);
+    return few ? tc_launch<T, 32, false>(p, map, box_rows, sms, s) : tc_launch<T, 64, false>(p, map, box_rows, sms, s);
 }
 
 } /* namespace */
@@ -1211,16 +1363,19 @@ cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, c
 extern "C" {
 
 /* Whether the tensor-core kernel takes the call: a 16-bit cache of whole
- * 128-column pairs and a rope part of at most a chunk, pages of whole 8-row
- * swizzle groups, and rows TMA and 16-byte loads can start at. Its boxes are
- * 64 columns by the returned number of rows (0: the other kernel's). */
+ * 64-column chunks, a rope part of at most one, and rows that 16-byte copies
+ * can start at (0: the other kernel's). Where pages are whole 8-row swizzle
+ * groups TMA loads them, in boxes of 64 columns by the returned number of
+ * rows; 1: they are copied row by row. */
 int wc_mla_tree_box(const waste_cuda_mla_tree_desc *d)
 {
     const uintptr_t addr = (uintptr_t)d->q | (uintptr_t)d->cache;
-    if (d->dtype == WASTE_CUDA_F32 || d->kl % 128 || d->rope > 64 || d->rope % 8 || d->page % 8 || (addr & 15) ||
-        d->row_stride % 8 || d->q_token_stride % 8 || d->q_head_stride % 8 || d->n_blocks < 1 ||
-        d->n_blocks > 0x7fffffff || d->row_stride * 2 * d->page >= ((size_t)1 << 40))
+    if (d->dtype == WASTE_CUDA_F32 || d->kl % 64 || d->rope > 64 || d->rope % 8 || (addr & 15) ||
+        d->row_stride % 8 || d->q_token_stride % 8 || d->q_head_stride % 8)
         return 0;
+    if (d->page % 8 || d->n_blocks < 1 || d->n_blocks > 0x7fffffff ||
+        d->row_stride * 2 * d->page >= ((size_t)1 << 40))
+        return d->n_blocks < 0xffffffffll / d->page ? 1 : 0;
     int r = 8;
     while (r < kTcKeys && d->page % (2 * r) == 0) r *= 2;
     return r;
@@ -1238,6 +1393,7 @@ int wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *map
     p.d = *d;
     p.err = err;
     const cudaStream_t s = (cudaStream_t)stream;
+    if (sms > kCombMax) sms = kCombMax;
     if (box_rows > 0)
         return (int)(d->dtype == WASTE_CUDA_F16 ? tc_launch<__half>(p, *map, box_rows, sms, s)
                                                 : tc_launch<__nv_bfloat16>(p, *map, box_rows, sms, s));

@@ -3403,7 +3403,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
     }
     int box = wc_mla_tree_box(d);
     CUtensorMap map;
-    if (box) {
+    memset(&map, 0, sizeof map);
+    if (box > 1) {
         const cuuint64_t dims[3] = { (cuuint64_t)(d->kl + d->rope), (cuuint64_t)d->page,
                                      (cuuint64_t)d->n_blocks };
         const cuuint64_t strides[2] = { d->row_stride * z, d->row_stride * z * (size_t)d->page };

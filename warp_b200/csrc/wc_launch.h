@@ -365,8 +365,9 @@ int    wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, vo
 int    wc_mla_rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, void *stream);
 size_t wc_mla_tree_ws_bytes(int kl, int sms);
 int    wc_mla_tree_box(const waste_cuda_mla_tree_desc *d);
-/* box_rows: wc_mla_tree_box's, with `map` the cache as {columns, rows of a
- * block, blocks} in boxes of {64, box_rows, 1} swizzled by 128 bytes; or 0. */
+/* box_rows: wc_mla_tree_box's; where it is above 1, `map` is the cache as
+ * {columns, rows of a block, blocks} in boxes of {64, box_rows, 1} swizzled by
+ * 128 bytes. */
 int    wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *map, int box_rows,
                           unsigned int *err, int sms, void *stream);
 int    wc_logits_launch(const waste_cuda_logits_desc *d, void *stream);
