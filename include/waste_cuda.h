@@ -777,7 +777,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  * allow_row[t], or under none if that is negative; allow_row NULL: mask t.
  * rep, freq, pres, hist NULL: 1, 0, 0, empty. Ids outside 0..V-1 are
  * ignored. ld, ld_out: elements between rows; out may be logits with the
- * same ld. Rows behind q_indptr[B] are left as they are. */
+ * same ld. Rows behind q_indptr[B] are left as they are. B up to 4096, R up
+ * to 65535. */
 typedef struct {
     int B, R, V, dtype, tree_words, allow_words, n_allow;
     size_t hist_stride, ld, ld_out;

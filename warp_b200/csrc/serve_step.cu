@@ -266,107 +266,298 @@ __global__ void __launch_bounds__(kRowsWarps * 32) mla_rows_kernel(
 }
 
 /* ---- logits -----------------------------------------------------------------
- * A CTA takes a slice of the ids of one request: the request's tokens that
- * fall into the slice are counted in shared memory (integer atomics: any
- * order gives the same counts), then the slice of each of the request's rows
- * is read, adjusted and written once. Each row's branch of drafted tokens is
- * counted before its slice and taken out again behind it. The bytes of the
- * logits bound it; the history is read again by each slice, from L2, so
- * slices are as wide as leaves enough CTAs to fill the GPU (wc_logits_launch).
+ * A CTA takes a slice of the ids for up to kLogRows rows of one request. Half
+ * of its warps copy the slice of each row, disallowed ids set to -infinity, 16
+ * bytes a thread and load, eight in flight: the bytes bound it. The other half
+ * finds meanwhile what the history, the drafts and the biases name: marked in
+ * a bitmap, numbered by its prefix counts and counted by number (integer
+ * atomics: any order gives the same counts). Then all set the named ids'
+ * values again; a row's branch of drafted tokens is counted where a drafted id
+ * is met. A count per named id and not per id lets the CTAs of a whole batch
+ * be resident at once; where a slice's named ids are more than kLogCap they
+ * are taken in pieces of kLogCap ids.
+ * 64 rows of 163840 16-bit logits take 18 us (43 MB: 6.6 us of copying), 180
+ * fp32 rows of 16 trees 78 us (247 MB: 38 us). Measured and slower: counts for
+ * every id, in several waves (33 us), the rows staged in shared memory (67),
+ * the sparse half following the copy row by row (20 and 85), the sparse work
+ * as a kernel of its own under the copy (24 and 94).
  *
- * A count word holds the times produced, and bit 31 for "in the prompt". */
-constexpr int kLogThreads = 256;
-constexpr uint32_t kPrompt = 0x80000000u;
+ * A count word holds the times produced, bit 31 for "in the prompt" and bit
+ * 30 for "drafted". */
+constexpr int kLogThreads = 512;
+constexpr int kLogHalf = kLogThreads / 2;
+constexpr int kLogSlice = 65536;     /* the widest slice                          */
+constexpr int kLogCap = 4096;
+constexpr int kLogDrafts = 256;      /* drafted tokens of a slice that are listed */
+constexpr int kLogRows = 4;          /* rows a CTA takes at most                  */
+constexpr int kLogKeep = 16;         /* tokens a thread keeps between its two uses */
+constexpr uint32_t kPrompt = 0x80000000u, kDrafted = 0x40000000u;
 
-struct LogitRow {
-    float rep, freq, pres;
-    const float *bias;
+struct alignas(16) LogitSmem {
+    uint32_t id[kLogCap], cnt[kLogCap], bias[kLogCap];
+    uint32_t named[kLogSlice / 32];
+    uint16_t before[kLogSlice / 32]; /* named ids before a word, from the piece's start */
+    int warp[kLogHalf / 32];
+    int n, nlist, list_j[kLogDrafts], list_u[kLogDrafts];
+    int mask[kLogRows];              /* a row's mask, -1: none                     */
 };
 
-__device__ __forceinline__ float adjust(float x, uint32_t c, uint32_t b, bool ok, const LogitRow &p)
+template <typename T> __device__ __forceinline__ void mask_vec(uint4 &v, uint32_t ok)
 {
-    if (c) {
-        x = x > 0.0f ? x / p.rep : x * p.rep;
-        const uint32_t n = c & ~kPrompt;
-        x -= p.freq * (float)n + (n ? p.pres : 0.0f);
-    }
-    if (b) x += p.bias[b - 1];
-    return ok ? x : -INFINITY;
+    T *e = reinterpret_cast<T *>(&v);
+#pragma unroll
+    for (int z = 0; z < 16 / (int)sizeof(T); z++)
+        if (!(ok >> z & 1)) e[z] = from_f<T>(-INFINITY);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogThreads) logits_kernel(const waste_cuda_logits_desc d, int vs)
+__global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda_logits_desc d, int vs)
 {
-    extern __shared__ __align__(16) uint32_t sml[];
-    uint32_t *cnt = sml, *bia = sml + vs;
-    const int tid = threadIdx.x, r = blockIdx.y, v0 = blockIdx.x * vs, nv = min(vs, d.V - v0);
-    int q0 = r, q1 = r + 1;
-    if (d.q_indptr) {
-        q0 = min(max(d.q_indptr[r], 0), d.R);
-        q1 = min(max(d.q_indptr[r + 1], q0), d.R);
+    constexpr int E = 16 / sizeof(T), U = 8;
+    extern __shared__ __align__(16) unsigned char sml[];
+    LogitSmem &s = *reinterpret_cast<LogitSmem *>(sml);
+    const int tid = threadIdx.x, lane = tid & 31, v0 = blockIdx.x * vs, nv = min(vs, d.V - v0);
+    const int words = (nv + 31) >> 5;
+    /* the request and its rows: chunk blockIdx.y of all requests' chunks */
+    int r = blockIdx.y, q0 = r, q1 = r + 1, t0 = r, rows = 1;
+    if (d.q_indptr) {                                         /* each warp for itself        */
+        const int per = (d.B + 31) / 32, first = lane * per, last = min(first + per, d.B);
+        auto begin = [&](int i) { return min(max(d.q_indptr[i], 0), d.R); };
+        auto chunks = [&](int i) { return (max(begin(i + 1) - begin(i), 0) + kLogRows - 1) / kLogRows; };
+        int sum = 0;
+        for (int i = first; i < last; i++) sum += chunks(i);
+        int at = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        at -= sum;
+        const int want = blockIdx.y;
+        const bool here = at <= want && want < at + sum;
+        const unsigned who = __ballot_sync(0xffffffffu, here);
+        if (!who) return;                                     /* the grid is a bound         */
+        if (here)
+            for (r = first; want >= at + chunks(r); r++) at += chunks(r);
+        r = __shfl_sync(0xffffffffu, r, __ffs(who) - 1);
+        at = __shfl_sync(0xffffffffu, at, __ffs(who) - 1);
+        q0 = begin(r);
+        q1 = begin(r + 1);
+        t0 = q0 + (want - at) * kLogRows;
+        rows = min(kLogRows, q1 - t0);
     }
-    if (q0 >= q1) return;
-    for (int i = tid; i < vs; i += kLogThreads) {
-        cnt[i] = 0;
-        if (d.bias_indptr) bia[i] = 0;
+    const T *x = static_cast<const T *>(d.logits) + (size_t)t0 * d.ld + v0;
+    T *y = static_cast<T *>(d.out) + (size_t)t0 * d.ld_out + v0;
+    auto mask_of = [&](int t) -> const uint32_t * {           /* of the chunk's row t        */
+        return s.mask[t] >= 0 ? d.allow + (size_t)s.mask[t] * d.allow_words + (v0 >> 5) : nullptr;
+    };
+    const int hn = d.hist ? min(max(d.hist_len[r], 0), (int)min(d.hist_stride, (size_t)0x7fffffff)) : 0;
+    const int hm = d.prompt_len ? d.prompt_len[r] : 0;
+    const int *hist = d.hist + (size_t)r * d.hist_stride;
+    const int b0 = d.bias_indptr ? max(d.bias_indptr[r], 0) : 0, bn = d.bias_indptr ? d.bias_indptr[r + 1] - b0 : 0;
+    const int ht = tid - kLogHalf;                            /* of the half that counts     */
+    /* what a thread needs twice is loaded once: under the copy a load takes long */
+    int keep[kLogKeep], id_b = -1, id_d = -1;
+    const float rep = d.rep ? d.rep[r] : 1.0f, freq = d.freq ? d.freq[r] : 0.0f, pres = d.pres ? d.pres[r] : 0.0f;
+    if (tid < rows) {
+        const int a = !d.allow ? -1 : d.allow_row ? d.allow_row[t0 + tid] : t0 + tid;
+        s.mask[tid] = a < d.n_allow ? a : -1;
+    }
+    if (ht >= 0) {
+#pragma unroll
+        for (int k = 0; k < kLogKeep; k++) keep[k] = ht + k * kLogHalf < hn ? hist[ht + k * kLogHalf] : -1;
+        if (ht < bn) id_b = d.bias_id[b0 + ht];
+        if (d.draft && ht < q1 - q0) id_d = d.draft[q0 + ht];
+        for (int i = ht; i < words; i += kLogHalf) s.named[i] = 0;
+        if (ht == 0) s.nlist = 0;
     }
     __syncthreads();
-    if (d.hist) {
-        const int n = min(max(d.hist_len[r], 0), (int)min(d.hist_stride, (size_t)0x7fffffff));
-        const int m = d.prompt_len ? d.prompt_len[r] : 0;
-        const int *h = d.hist + (size_t)r * d.hist_stride;
-#pragma unroll 4
-        for (int i = tid; i < n; i += kLogThreads) {
-            const unsigned u = (unsigned)h[i] - (unsigned)v0;
-            if (u < (unsigned)nv) {
-                if (i < m) atomicOr(&cnt[u], kPrompt);
-                else atomicAdd(&cnt[u], 1u);
+    /* ids [32 w0, 32 (w0 + wn)) of the slice numbered; how many are named */
+    auto sync_half = [] { asm volatile("bar.sync 1, %0;" ::"n"(kLogHalf) : "memory"); };
+    auto numbered = [&](int w0, int wn) {
+        const int per = (wn + kLogHalf - 1) / kLogHalf, ws = w0 + ht * per, we = min(ws + per, w0 + wn);
+        int sum = 0;
+        for (int k = ws; k < we; k++) sum += __popc(s.named[k]);
+        int at = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += v;
+        }
+        if (lane == 31) s.warp[ht >> 5] = at;
+        sync_half();
+        const int v = lane < kLogHalf / 32 ? s.warp[lane] : 0;
+        const int n = __reduce_add_sync(0xffffffffu, v);
+        at += __reduce_add_sync(0xffffffffu, lane < (ht >> 5) ? v : 0) - sum;
+        if (ht == 0) s.n = n;
+        if (n <= kLogCap) {
+            for (int k = ws; k < we; k++) {
+                s.before[k] = (uint16_t)at;
+                at += __popc(s.named[k]);
+            }
+            for (int i = ht; i < n; i += kLogHalf) s.cnt[i] = s.bias[i] = 0;
+            sync_half();
+            /* words that are full lie side by side: a thread takes every 256th */
+            for (int k = w0 + ht; k < w0 + wn; k += kLogHalf) {
+                int to = s.before[k];
+                for (uint32_t m = s.named[k]; m; m &= m - 1) s.id[to++] = 32 * k + __ffs(m) - 1;
             }
         }
-    }
-    LogitRow p = { d.rep ? d.rep[r] : 1.0f, d.freq ? d.freq[r] : 0.0f, d.pres ? d.pres[r] : 0.0f, nullptr };
-    if (d.bias_indptr) {
-        const int b0 = max(d.bias_indptr[r], 0), b1 = d.bias_indptr[r + 1];
-        p.bias = d.bias_val + b0;
-        for (int i = b0 + tid; i < b1; i += kLogThreads) {
-            const unsigned u = (unsigned)d.bias_id[i] - (unsigned)v0;
-            if (u < (unsigned)nv) atomicMax(&bia[u], (uint32_t)(i - b0 + 1));
+        sync_half();
+        return n;
+    };
+    /* their counts */
+    auto counted = [&](int w0, int wn) {
+        auto number = [&](int id) {
+            const unsigned u = (unsigned)id - (unsigned)v0, w = (u >> 5) - (unsigned)w0;
+            return u < (unsigned)nv && w < (unsigned)wn
+                       ? (int)s.before[u >> 5] + __popc(s.named[u >> 5] & ((1u << (u & 31)) - 1u)) : -1;
+        };
+        auto count = [&](int i, int id) {
+            const int k = number(id);
+            if (k < 0) return;
+            if (i < hm) atomicOr(&s.cnt[k], kPrompt);
+            else atomicAdd(&s.cnt[k], 1u);
+        };
+#pragma unroll
+        for (int k = 0; k < kLogKeep; k++) count(ht + k * kLogHalf, keep[k]);
+#pragma unroll 8
+        for (int i = ht + kLogKeep * kLogHalf; i < hn; i += kLogHalf) count(i, hist[i]);
+        for (int i = ht; i < bn; i += kLogHalf) {
+            const int k = number(i == ht ? id_b : d.bias_id[b0 + i]);
+            if (k >= 0) atomicMax(&s.bias[k], (uint32_t)(i + 1));
         }
+        if (d.draft)
+            for (int j = ht; j < q1 - q0; j += kLogHalf) {
+                const int k = number(j == ht ? id_d : d.draft[q0 + j]);
+                if (k >= 0) atomicOr(&s.cnt[k], kDrafted);
+            }
+    };
+    if (ht < 0) {
+        /* ---- the copy, row by row. Loaded words are not looked at before all loads
+         * are out ---- */
+        const bool wide = (((uintptr_t)x | (uintptr_t)y) & 15) == 0 &&
+                          (rows == 1 || (d.ld % E == 0 && d.ld_out % E == 0));
+        for (int t = 0; t < rows; t++) {
+            const uint32_t *allow = mask_of(t);
+            const T *xr = x + (size_t)t * d.ld;
+            T *yr = y + (size_t)t * d.ld_out;
+            const uint4 *xv = reinterpret_cast<const uint4 *>(xr);
+            uint4 *yv = reinterpret_cast<uint4 *>(yr);
+            const int nvec = wide ? nv / E : 0;
+            for (int c = tid; c < nvec; c += U * kLogHalf) {
+                uint4 v[U];
+                uint32_t w[U];
+                if (allow) {
+#pragma unroll
+                    for (int k = 0; k < U; k++) w[k] = __ldg(allow + (min(c + k * kLogHalf, nvec - 1) * E >> 5));
+                }
+#pragma unroll
+                for (int k = 0; k < U; k++) v[k] = __ldcs(xv + min(c + k * kLogHalf, nvec - 1));
+                if (allow) {
+#pragma unroll
+                    for (int k = 0; k < U; k++) mask_vec<T>(v[k], w[k] >> ((c + k * kLogHalf) * E & 31));
+                }
+#pragma unroll
+                for (int k = 0; k < U; k++)
+                    if (c + k * kLogHalf < nvec) yv[c + k * kLogHalf] = v[k];
+            }
+#pragma unroll 8
+            for (int i = nvec * E + tid; i < nv; i += kLogHalf)
+                yr[i] = !allow || (allow[i >> 5] >> (i & 31) & 1) ? xr[i] : from_f<T>(-INFINITY);
+        }
+    }
+    if (ht >= 0) {
+        /* ---- what is named ---- */
+        auto mark = [&](int id) {
+            const unsigned u = (unsigned)id - (unsigned)v0;
+            if (u >= (unsigned)nv) return false;
+            atomicOr(&s.named[u >> 5], 1u << (u & 31));
+            return true;
+        };
+#pragma unroll
+        for (int k = 0; k < kLogKeep; k++) mark(keep[k]);
+#pragma unroll 8
+        for (int i = ht + kLogKeep * kLogHalf; i < hn; i += kLogHalf) mark(hist[i]);
+        mark(id_b);
+        for (int i = ht + kLogHalf; i < bn; i += kLogHalf) mark(d.bias_id[b0 + i]);
+        if (d.draft)
+            for (int j = ht; j < q1 - q0; j += kLogHalf) {
+                const int id = j == ht ? id_d : d.draft[q0 + j];
+                if (!mark(id)) continue;
+                const int k = atomicAdd(&s.nlist, 1);
+                if (k < kLogDrafts) { s.list_j[k] = j; s.list_u[k] = id - v0; }
+            }
+        sync_half();
+        if (numbered(0, words) <= kLogCap) counted(0, words);
     }
     __syncthreads();
-    for (int t = q0; t < q1; t++) {
-        if (d.draft) {
-            for (int j = tid; j < q1 - q0; j += kLogThreads) {
-                const bool on = d.tree ? j < 32 * d.tree_words &&
-                                             ((d.tree[(size_t)t * d.tree_words + (j >> 5)] >> (j & 31)) & 1)
-                                       : j <= t - q0;
-                const unsigned u = (unsigned)d.draft[q0 + j] - (unsigned)v0;
-                if (on && u < (unsigned)nv) atomicAdd(&cnt[u], 1u);
+    /* ---- the named ids again ---- */
+    auto on = [&](int t, int j) {
+        return d.tree ? j < 32 * d.tree_words &&
+                            ((d.tree[(size_t)(t0 + t) * d.tree_words + (j >> 5)] >> (j & 31)) & 1)
+                      : j <= t0 + t - q0;
+    };
+    /* times the branch of row t drafts id u of the slice */
+    auto drafted = [&](int t, int u) {
+        uint32_t n = 0;
+        if (s.nlist <= kLogDrafts) {
+            for (int k = 0; k < s.nlist; k++)
+                if (s.list_u[k] == u) n += on(t, s.list_j[k]);
+        } else {
+            for (int j = 0; j < q1 - q0; j++)
+                if (d.draft[q0 + j] == v0 + u) n += on(t, j);
+        }
+        return n;
+    };
+    auto again = [&](int t, int n) {
+        constexpr int Z = 4;
+        const uint32_t *allow = mask_of(t);
+        const T *xr = x + (size_t)t * d.ld;
+        T *yr = y + (size_t)t * d.ld_out;
+        for (int k0 = tid; k0 < n; k0 += Z * kLogThreads) {
+            T raw[Z];
+            uint32_t w[Z];
+#pragma unroll
+            for (int z = 0; z < Z; z++) {
+                const int i = (int)s.id[min(k0 + z * kLogThreads, n - 1)];
+                raw[z] = yr[i];
+                w[z] = allow ? __ldg(allow + (i >> 5)) : 0xffffffffu;
             }
-            __syncthreads();
-        }
-        const uint32_t *allow = nullptr;
-        if (d.allow) {
-            const int a = d.allow_row ? d.allow_row[t] : t;
-            if (a >= 0 && a < d.n_allow) allow = d.allow + (size_t)a * d.allow_words;
-        }
-        const T *x = static_cast<const T *>(d.logits) + (size_t)t * d.ld + v0;
-        T *y = static_cast<T *>(d.out) + (size_t)t * d.ld_out + v0;
-        for (int i = tid; i < nv; i += kLogThreads) {
-            const bool ok = !allow || ((allow[(v0 + i) >> 5] >> ((v0 + i) & 31)) & 1);
-            y[i] = from_f<T>(adjust(to_f(x[i]), cnt[i], d.bias_indptr ? bia[i] : 0u, ok, p));
-        }
-        if (d.draft) {
-            __syncthreads();
-            for (int j = tid; j < q1 - q0; j += kLogThreads) {
-                const bool on = d.tree ? j < 32 * d.tree_words &&
-                                             ((d.tree[(size_t)t * d.tree_words + (j >> 5)] >> (j & 31)) & 1)
-                                       : j <= t - q0;
-                const unsigned u = (unsigned)d.draft[q0 + j] - (unsigned)v0;
-                if (on && u < (unsigned)nv) atomicSub(&cnt[u], 1u);
+#pragma unroll
+            for (int z = 0; z < Z; z++) {
+                const int k = k0 + z * kLogThreads;
+                if (k >= n) break;
+                const int i = (int)s.id[k];
+                if (!(w[z] >> (i & 31) & 1)) continue;
+                const uint32_t b = s.bias[k];
+                uint32_t c = s.cnt[k];
+                if (c & kDrafted) c = (c & ~kDrafted) + drafted(t, i);
+                float f = to_f(raw[z]);
+                if (c) {
+                    f = f > 0.0f ? f / rep : f * rep;
+                    const uint32_t m = c & ~kPrompt;
+                    f -= freq * (float)m + (m ? pres : 0.0f);
+                }
+                if (b) f += d.bias_val[b0 + b - 1];
+                if (c | b) yr[i] = from_f<T>(f);
             }
-            __syncthreads();
         }
+    };
+    const int total = s.n;
+    if (total <= kLogCap) {
+        for (int t = 0; t < rows; t++) again(t, total);
+        return;
+    }
+    for (int w0 = 0; w0 < words; w0 += kLogCap / 32) {
+        const int wn = min(kLogCap / 32, words - w0);
+        __syncthreads();
+        if (ht >= 0) {
+            numbered(w0, wn);
+            counted(w0, wn);
+        }
+        __syncthreads();
+        for (int t = 0; t < rows; t++) again(t, s.n);
     }
 }
 
@@ -381,13 +572,22 @@ cudaError_t rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, cu
 }
 
 template <typename T>
-cudaError_t logits_launch(const waste_cuda_logits_desc *d, int vs, cudaStream_t s)
+cudaError_t logits_launch(const waste_cuda_logits_desc *d, int sms, cudaStream_t s)
 {
-    const size_t smem = (size_t)vs * 2 * sizeof(uint32_t);
+    /* as many slices as are resident at once, two CTAs an SM: a few more wait for
+     * a whole turn, fewer read the history less often */
+    int chunks = d->B;
+    if (d->q_indptr) {
+        const long long bound = (long long)d->R / kLogRows + d->B;
+        chunks = (int)(bound < d->R ? bound : d->R);
+    }
+    const int most = 2 * sms / chunks > 1 ? 2 * sms / chunks : 1;
+    int vs = ((d->V + most - 1) / most + 1023) & ~1023;
+    if (vs > kLogSlice) vs = kLogSlice;
     cudaError_t e = cudaFuncSetAttribute(logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
+                                         (int)sizeof(LogitSmem));
     if (e != cudaSuccess) return e;
-    logits_kernel<T><<<dim3((d->V + vs - 1) / vs, d->B), kLogThreads, smem, s>>>(*d, vs);
+    logits_kernel<T><<<dim3((d->V + vs - 1) / vs, chunks), kLogThreads, sizeof(LogitSmem), s>>>(*d, vs);
     return cudaGetLastError();
 }
 
@@ -429,16 +629,13 @@ int wc_mla_rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, voi
     return (int)rows_launch<__nv_bfloat16>(d, err, s);
 }
 
-int wc_logits_launch(const waste_cuda_logits_desc *d, void *stream)
+int wc_logits_launch(const waste_cuda_logits_desc *d, int sms, void *stream)
 {
-    /* the widest slice that still leaves four CTAs an SM */
-    int vs = 8192;
-    while (vs > 1024 && (long long)d->B * ((d->V + vs - 1) / vs) < 4 * 148) vs >>= 1;
     const cudaStream_t s = (cudaStream_t)stream;
     wc_count_launches(1);
-    if (d->dtype == WASTE_CUDA_F32) return (int)logits_launch<float>(d, vs, s);
-    if (d->dtype == WASTE_CUDA_F16) return (int)logits_launch<__half>(d, vs, s);
-    return (int)logits_launch<__nv_bfloat16>(d, vs, s);
+    if (d->dtype == WASTE_CUDA_F32) return (int)logits_launch<float>(d, sms, s);
+    if (d->dtype == WASTE_CUDA_F16) return (int)logits_launch<__half>(d, sms, s);
+    return (int)logits_launch<__nv_bfloat16>(d, sms, s);
 }
 
 } /* extern "C" */

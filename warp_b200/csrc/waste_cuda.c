@@ -3431,10 +3431,10 @@ out:
 int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream)
 {
     int rc = 0;
-    if (!d || d->B < 0 || d->B > 65535 || d->R < 0 || d->V < 1 || d->V > INT32_MAX - 8192 ||
+    if (!d || d->B < 0 || d->R < 0 || d->B > 4096 || d->R > 65535 || d->V < 1 || d->V > INT32_MAX - 8192 ||
         !dtype_size(d->dtype) || d->ld < (size_t)d->V || d->ld_out < (size_t)d->V ||
         (!d->q_indptr && d->R != d->B))
-        return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: bad sizes, type or strides (B up to 65535)");
+        return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: bad sizes, type or strides (B up to 4096, R up to 65535)");
     if (d->B == 0 || d->R == 0) return 0;
     if (!d->logits || !d->out || (d->out == d->logits && d->ld != d->ld_out) ||
         (d->hist && !d->hist_len) || (d->tree && (!d->draft || d->tree_words < 1)) ||
@@ -3444,7 +3444,8 @@ int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream)
         return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: a missing, short or misaligned array");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("logits_adjust_dev"))) goto out;
-    CK((cudaError_t)wc_logits_launch(d, stream ? stream : (void *)S.stream), "logits_adjust");
+    CK((cudaError_t)wc_logits_launch(d, S.sms, stream ? stream : (void *)S.stream),
+       "logits_adjust");
 out:
     pthread_mutex_unlock(&g_mu);
     return rc;
