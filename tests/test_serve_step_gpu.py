@@ -341,6 +341,14 @@ ATTN = {
     "kl_odd": ("f16", 3, (77, 5), 16, [90], [3], None),
     "kl_1": ("f32", 2, (1, 0), 4, [9], [2], None),
     "rope_128": ("bf16", 8, (512, 128), 64, [150], [2], None),
+    # several key tiles a CTA, tiles cut between CTAs, of one, two and three tokens' rows
+    "many_singles": ("bf16", 32, KIMI, 64, [900 - 37 * r for r in range(24)] * 2, [1] * 48, None),
+    "many_pairs": ("f16", 32, KIMI, 32, [1500 - 90 * r for r in range(16)] * 2, [2] * 32, 1),
+    "many_drafts": ("bf16", 32, KIMI, 64, [2900 - 200 * r for r in range(12)], [5, 3, 4, 9] * 3, 1),
+    "many_chunks": ("f16", 32, KIMI, 16, [1500, 0, 900, 1200], [40, 100, 33, 20], None),
+    "many_narrow": ("bf16", 64, (192, 32), 64, [2600 - 170 * r for r in range(12)], [3, 2] * 6, 1),
+    "many_small_pages": ("bf16", 32, KIMI, 4, [1300 - 100 * r for r in range(12)], [3, 1, 2, 4] * 3, 1),
+    "many_f32": ("f32", 16, (128, 16), 16, [1700 - 100 * r for r in range(16)], [1, 2] * 8, 1),
     "f32_engine": ("f32", 32, KIMI, 64, [500], [1], None),
     "f32_tree": ("f32", 32, KIMI, 16, [90, 0, 200], [5, 3, 1], 1),
     "f32_small": ("f32", 4, (64, 16), 16, [33, 64, 0], [2, 1, 4], None),
@@ -394,7 +402,8 @@ def test_attn_unserved_and_empty(cuda_lib, name):
     assert torch.equal(a.go, b.go)
 
 
-@pytest.mark.parametrize("name", ["tree", "f32_tree", "pages_24", "pages_5", "kl_128", "tile_edges"])
+@pytest.mark.parametrize("name", ["tree", "f32_tree", "pages_24", "pages_5", "kl_128", "tile_edges", "many_singles",
+                                  "many_pairs", "many_drafts", "many_small_pages", "many_f32"])
 def test_attn_what_is_not_seen(cuda_lib, name):
     """NaN and infinities in rows behind a request's last, in blocks of no
     request, behind the latents of a row, and in a drafted row that only some
@@ -431,7 +440,7 @@ def test_attn_what_is_not_seen(cuda_lib, name):
     assert bool((d <= to[clean]).all())
 
 
-@pytest.mark.parametrize("name", ["tree", "long", "f32_tree"])
+@pytest.mark.parametrize("name", ["tree", "long", "f32_tree", "many_singles", "many_pairs", "many_drafts", "many_f32"])
 def test_attn_extreme_scores(cuda_lib, name):
     """Scores of some thousands, of both signs, rising along the cache: the
     softmax stays finite and is the largest key's."""
@@ -498,7 +507,8 @@ def test_attn_bad_blocks(cuda_lib, name):
     assert wb.device_errors() == wb.DERR_BAD_BLOCK
 
 
-@pytest.mark.parametrize("name", ["long", "tree", "f32_tree", "prompt"])
+@pytest.mark.parametrize("name", ["long", "tree", "f32_tree", "prompt", "many_singles", "many_pairs", "many_drafts",
+                                  "many_chunks", "many_f32"])
 def test_attn_same_every_time(cuda_lib, name):
     """The same bits from every call, and beside calls on another stream."""
     a, b = attn_case(cuda_lib, name).put(), attn_case(cuda_lib, "ragged").put()

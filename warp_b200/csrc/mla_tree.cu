@@ -508,23 +508,25 @@ template <int N> struct TcCfg {
     static constexpr int off_ctl = off_q + 9 * N * 128;
 };
 
-struct TcCtl {
+template <int N> struct TcCtl {
     uint64_t pair_full[kMaxPairs], pair_empty[kMaxPairs];
     uint64_t rope_full, rope_empty, q_full, s_full, p_ready, o_done, drain;
     uint32_t tmem;
     volatile int dead;
     WalkSmem walk;
-    float mx[4][4][16];              /* [quarter][quadrant][column]                  */
-    float col[4][2][16];             /* [quarter] two values of each column           */
-    long long qoff[64], ooff[2][64]; /* a tile row's elements in q (-1: no row) and o */
-    int tok[64];                     /* its token in the request                     */
+    float mx[4][4][N / 4];            /* [quarter][quadrant][column]                  */
+    alignas(16) float col[4][2][N / 4]; /* [quarter] a factor and the reference of each column */
+    long long qoff[N], ooff[2][N];   /* a tile row's elements in q (-1: no row) and o */
+    int tok[N];                      /* its token in the request                     */
     uint32_t krow[kTcKeys];          /* a key's row of the cache, without TMA         */
     unsigned char nan_row[kTcKeys];  /* a new row that holds no finite number        */
-    Seg seg[2];                      /* the softmax warps' segment and the next       */
-    int more[2];
+    /* the softmax warps' segments: the next is found while some are at the last */
+    Seg seg[3];
+    int more[3];
 };
 
-__device__ __forceinline__ bool tc_wait(TcCtl &c, uint64_t *bar, uint32_t parity, unsigned int *err)
+template <int N>
+__device__ __forceinline__ bool tc_wait(TcCtl<N> &c, uint64_t *bar, uint32_t parity, unsigned int *err)
 {
     for (int i = 0; i < kMbarLimit; i++) {
         uint32_t done;
@@ -598,8 +600,8 @@ template <int NC> __device__ __forceinline__ void tm_ld(float *v, uint32_t addr)
                      : "r"(addr + k));
     if (NC == 8)
         asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]),
-                       "=r"(u[6]), "=r"(u[7]) : "r"(addr));
+                     : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]),
+                       "=r"(u[5]), "=r"(u[6]), "=r"(u[7]) : "r"(addr));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 template <int NC> __device__ __forceinline__ void tm_st(const float *v, uint32_t addr)
@@ -615,8 +617,8 @@ template <int NC> __device__ __forceinline__ void tm_st(const float *v, uint32_t
                        "r"(u[k + 14]), "r"(u[k + 15]) : "memory");
     if (NC == 8)
         asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                     ::"r"(addr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]),
-                       "r"(u[6]), "r"(u[7]) : "memory");
+                     ::"r"(addr), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]),
+                       "r"(u[5]), "r"(u[6]), "r"(u[7]) : "memory");
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
 
@@ -679,7 +681,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
     constexpr float kBias = kF16 ? 8.0f : 0.0f;
     extern __shared__ unsigned char smt[];
     unsigned char *sm = smt + ((1024 - (smem_u32(smt) & 1023)) & 1023);
-    TcCtl &c = *reinterpret_cast<TcCtl *>(sm + Cfg::off_ctl);
+    TcCtl<N> &c = *reinterpret_cast<TcCtl<N> *>(sm + Cfg::off_ctl);
     const waste_cuda_mla_tree_desc &d = p.d;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int npair = (d.kl + 127) / 128, nchunk = d.kl / 64 + (d.rope > 0), H = d.heads;
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         blk = d.block_table[(size_t)g.q.r * d.max_blocks + b];
                         if (blk < 0 || blk >= d.n_blocks) {
                             atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
-                            blk = (int)d.n_blocks;            /* reads zeros                 */
+                            blk = (int)d.n_blocks;                /* reads zeros                 */
                         }
                     }
                     const uint32_t chunk_tx = (uint32_t)(nbox * box_rows) * 128u;
@@ -834,40 +836,49 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
             const uint32_t q_lo = desc_lo(sm0 + Cfg::off_q, 16), p_lo = desc_lo(sm0 + Cfg::off_p, 16);
             const uint32_t r_lo = desc_lo(sm0 + Cfg::off_rope, 16);
             const int rope_steps = (d.rope + 15) / 16;
-            int slot0 = 0, par0 = 0;                          /* the tile's first pair       */
+            int slot = 0, par = 0;                            /* the next pair in the ring   */
             int unit = 0, segs = 0;
             bool ok = true;
+            auto step = [&]() {
+                if (++slot == Cfg::pairs) { slot = 0; par ^= 1; }
+            };
+            /* S^T of unit u, whose pairs come next in the ring */
+            auto scores = [&](int u) {
+                tc_fence_after();
+                for (int j = 0; j < npair && ok; j++) {
+                    ok = tc_wait(c, &c.pair_full[slot], par, p.err);
+                    if (!ok) return;
+                    const uint32_t a = k_lo + slot * (kPairBytes / 16), b = q_lo + j * (2 * N * 128 / 16);
+                    const int steps = odd && j == npair - 1 ? 4 : 8;
+#pragma unroll
+                    for (int k = 0; k < 8; k++)
+                        if (k < steps)
+                            tc_mma<kHi, kHi>(tm_s, a + (k >> 2) * (kTcKeys * 128 / 16) + (k & 3) * 2,
+                                             b + (k >> 2) * (N * 128 / 16) + (k & 3) * 2, id_s, (j | k) != 0);
+                    step();
+                }
+                if (d.rope > 0 && ok) {
+                    ok = tc_wait(c, &c.rope_full, u & 1, p.err);
+                    if (!ok) return;
+                    const uint32_t b = q_lo + (d.kl / 64) * (N * 128 / 16);
+                    for (int k = 0; k < rope_steps; k++)
+                        tc_mma<kHi, kHi>(tm_s, r_lo + k * 2, b + k * 2, id_s, 1u);
+                }
+                if (!ok) return;
+                tc_commit(&c.s_full);
+                if (N != 64) tc_commit(&c.rope_empty);
+            };
             while (ok && walk_next(p, w, g)) {
                 if (g.k0 == g.k1) continue;
                 ok = tc_wait(c, &c.q_full, segs & 1, p.err);
                 for (int kt = g.k0; kt < g.k1 && ok; kt++, unit++) {
-                    int slot = slot0, par = par0;
-                    tc_fence_after();
-                    for (int j = 0; j < npair && ok; j++) {
-                        ok = tc_wait(c, &c.pair_full[slot], par, p.err);
-                        if (!ok) break;
-                        const uint32_t a = k_lo + slot * (kPairBytes / 16), b = q_lo + j * (2 * N * 128 / 16);
-                        const int steps = odd && j == npair - 1 ? 4 : 8;
-#pragma unroll
-                        for (int k = 0; k < 8; k++)
-                            if (k < steps) tc_mma<kHi, kHi>(tm_s, a + (k >> 2) * (kTcKeys * 128 / 16) + (k & 3) * 2,
-                                             b + (k >> 2) * (N * 128 / 16) + (k & 3) * 2, id_s, (j | k) != 0);
-                        if (++slot == Cfg::pairs) { slot = 0; par ^= 1; }
-                    }
-                    if (d.rope > 0 && ok) {
-                        ok = tc_wait(c, &c.rope_full, unit & 1, p.err);
-                        if (!ok) break;
-                        const uint32_t b = q_lo + (d.kl / 64) * (N * 128 / 16);
-                        for (int k = 0; k < rope_steps; k++)
-                            tc_mma<kHi, kHi>(tm_s, r_lo + k * 2, b + k * 2, id_s, 1u);
-                    }
-                    if (!ok) break;
-                    tc_commit(&c.s_full);
-                    if (N != 64) tc_commit(&c.rope_empty);
-                    ok = tc_wait(c, &c.p_ready, unit & 1, p.err);
+                    const int slot0 = slot, par0 = par;       /* of the tile's pairs, held   */
+                    scores(unit);
+                    if (ok) ok = tc_wait(c, &c.p_ready, unit & 1, p.err);
                     if (!ok) break;
                     tc_fence_after();
                     slot = slot0;
+                    par = par0;
                     for (int j = 0; j < npair; j++) {
                         const uint32_t a = v_lo + slot * (kPairBytes / 16);
 #pragma unroll
@@ -875,11 +886,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                             tc_mma<kHi, kHiP>(tmem + j * N, a + k * (2048 / 16), p_lo + k * (16 * Cfg::p_row / 16),
                                               id_o, kt > g.k0 || k > 0);
                         tc_commit(&c.pair_empty[slot]);
-                        if (++slot == Cfg::pairs) slot = 0;
+                        step();
                     }
                     if (N == 64) tc_commit(&c.rope_empty);
-                    slot0 += npair;
-                    if (slot0 >= Cfg::pairs) { slot0 -= Cfg::pairs; par0 ^= 1; }
                 }
                 if (ok) tc_commit(&c.o_done);
                 segs++;
@@ -896,20 +905,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         const int st = tid - 64, quarter = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = quarter * NC;
         const uint32_t tm_lane = (uint32_t)(quad * 32) << 16;
         const float scale2 = d.scale * 1.4426950408889634f;
-        float(*mine)[16] = c.col[quarter];                    /* the 4 warps write the same  */
-        float(*sx)[16] = c.mx[quarter];
-        int unit = 0, segs = 0, slot0 = 0, par0 = 0;
+        float(*mine)[NC] = c.col[quarter];                    /* the 4 warps write the same  */
+        float(*sx)[NC] = c.mx[quarter];
+        int unit = 0, segs = 0, pos = 0;                      /* pos: the segment's first pair */
         /* tables of segment i's rows, and its query tile: swizzled 128-byte rows,
          * zeros past its rows and columns, a row's eight 16-byte units of a chunk
          * to eight threads */
-        auto tables = [&](int i) {
+        auto tables = [&](int i, int o) {                     /* o: which of the offsets     */
             const Seg &g = c.seg[i];
             if (st < N) {
                 const int at = g.row0 + st, tok = at / H, h = at - tok * H;
                 const bool in = st < g.rows;
                 c.tok[st] = in ? tok : 0x3fffffff;
                 c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * d.q_head_stride : -1;
-                c.ooff[i][st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
+                c.ooff[o][st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
             }
         };
         auto queries = [&](int i) {
@@ -942,17 +951,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         bar_named(5, kTcSoft);                                /* every role has the start    */
         if (st == 0) next(0);
         bar_named(5, kTcSoft);
-        tables(0);
+        tables(0, 0);
         bar_named(5, kTcSoft);
         queries(0);
-        for (int cur = 0;; cur ^= 1) {
+        for (int cur = 0, which = 0;; which ^= 1) {
+            const int then = cur == 2 ? 0 : cur + 1;
             const Seg &g = c.seg[cur];
-            if (st == 0) next(cur ^ 1);                       /* while the first tile loads  */
+            if (st == 0) next(then);                          /* while the first tile loads  */
             const bool whole = g.first && g.last;
             const int slot = part_slot(g);
-            float l[NC], ref[NC];                             /* ref less the fp16 bias      */
+            /* the references (less the fp16 bias) lie in mine[1] */
+            if (lane < NC) mine[1][lane] = kNone;
+            __syncwarp();
+            float l[NC];
 #pragma unroll
-            for (int i = 0; i < NC; i++) { l[i] = 0.0f; ref[i] = kNone; }
+            for (int i = 0; i < NC; i++) l[i] = 0.0f;
             for (int kt = g.k0; kt < g.k1; kt++, unit++) {
                 const bool tail = kt * kTcKeys + kTcKeys > g.q.ctx || kt * kTcKeys + kTcKeys > g.vis;
                 float x[NC];
@@ -961,16 +974,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 tm_ld<NC>(x, tm_s + tm_lane + c0);
                 uint32_t seen = 0xffffffffu;                  /* columns that see this key   */
                 bool bad = false;
+                const int key = kt * kTcKeys + key_row;
                 if (tail) {
                     /* rows past the request's are zeros to the second product, and so is
                      * a new row that holds a NaN or an infinity: who sees it gets NaN
                      * weights, who does not is not touched. A quarter takes a pair. */
-                    const int key = kt * kTcKeys + key_row;
-                    int sl = slot0 + quarter, pr = par0;
-                    if (sl >= Cfg::pairs) { sl -= Cfg::pairs; pr ^= 1; }
+                    const int at = pos + (kt - g.k0) * npair + quarter, sl = at % Cfg::pairs;
                     unsigned char *mem = sm + sl * kPairBytes + key_row * 128;
                     const int units = odd && quarter == npair - 1 ? 8 : 16;
-                    if (quarter < npair) tc_wait(c, &c.pair_full[sl], pr, p.err);
+                    if (quarter < npair) tc_wait(c, &c.pair_full[sl], (at / Cfg::pairs) & 1, p.err);
                     if (quarter == 0) c.nan_row[key_row] = 0;
                     bar_named(5, kTcSoft);
                     if (quarter < npair && key >= g.q.ctx && key < g.vis) {
@@ -1004,29 +1016,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                             see = in && (nj < 0 || (tok < g.q.n && sees(p, g.q, tok, nj)));
                         }
                         if (see) seen |= 1u << i;
-                        if (bad) x[i] = __int_as_float(0x7fc00000);
                     }
                 }
-                float y[NC], top = -INFINITY;
+                /* the exponents: x becomes x * scale2 - reference, masked ones -infinity */
+                auto exponents = [&]() {
 #pragma unroll
-                for (int i = 0; i < NC; i++) y[i] = fmaf(x[i], scale2, -ref[i]);
-                if (tail) {
+                    for (int i = 0; i < NC; i += 4) {
+                        const float4 r = *reinterpret_cast<const float4 *>(&mine[1][i]);
+                        x[i] = fmaf(x[i], scale2, -r.x);
+                        x[i + 1] = fmaf(x[i + 1], scale2, -r.y);
+                        x[i + 2] = fmaf(x[i + 2], scale2, -r.z);
+                        x[i + 3] = fmaf(x[i + 3], scale2, -r.w);
+                    }
+                    if (tail) {
 #pragma unroll
-                    for (int i = 0; i < NC; i++)
-                        if (!(seen >> i & 1)) y[i] = -INFINITY;
-                }
+                        for (int i = 0; i < NC; i++)
+                            x[i] = !(seen >> i & 1) ? -INFINITY : bad ? __int_as_float(0x7fc00000) : x[i];
+                    }
+                };
+                exponents();
+                float top = x[0];
 #pragma unroll
-                for (int i = 0; i < NC; i++) top = fmaxf(top, y[i]);
+                for (int i = 1; i < NC; i++) top = fmaxf(top, x[i]);
                 if (bar_any(1 + quarter, top > kBias + kLazy)) {
-                    float mx = -INFINITY, r = kNone;          /* of column c0 + lane % NC     */
+                    tm_ld<NC>(x, tm_s + tm_lane + c0);
+                    float mx = -INFINITY;                     /* of column c0 + lane         */
 #pragma unroll
                     for (int i = 0; i < NC; i++) {
                         const float m = warp_max(seen >> i & 1 ? x[i] * scale2 : -INFINITY);
-                        if (lane % NC == i) { mx = m; r = ref[i]; }
+                        if (lane == i) mx = m;
                     }
+                    const int lc = min(lane, NC - 1);
                     if (lane < NC) sx[quad][lane] = mx;
+                    float r = mine[1][lc];
                     bar_named(1 + quarter, 128);
-                    mx = fmaxf(fmaxf(sx[0][lane % NC], sx[1][lane % NC]), fmaxf(sx[2][lane % NC], sx[3][lane % NC]));
+                    mx = fmaxf(fmaxf(sx[0][lc], sx[1][lc]), fmaxf(sx[2][lc], sx[3][lc]));
                     float a = 1.0f;
                     if (mx > r + (kBias + kLazy)) {
                         a = ex2(r - (mx - kBias));
@@ -1035,20 +1059,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     if (lane < NC) { mine[0][lane] = a; mine[1][lane] = r; }
                     bar_named(1 + quarter, 128);              /* and sx is read              */
 #pragma unroll
-                    for (int i = 0; i < NC; i++) {
-                        l[i] *= mine[0][i];
-                        ref[i] = mine[1][i];
-                        y[i] = seen >> i & 1 ? fmaf(x[i], scale2, -ref[i]) : -INFINITY;
-                    }
+                    for (int i = 0; i < NC; i++) l[i] *= mine[0][i];
+                    exponents();
                     if (kt > g.k0) {
                         /* the products before are done: S's commit followed them */
 #pragma unroll 1
                         for (int j = 0; j < npair; j++) {
-                            float o[NC];
-                            tm_ld<NC>(o, tmem + tm_lane + j * N + c0);
+#pragma unroll 1
+                            for (int h = 0; h < NC; h += 8) {
+                                float o[8];
+                                tm_ld<8>(o, tmem + tm_lane + j * N + c0 + h);
 #pragma unroll
-                            for (int i = 0; i < NC; i++) o[i] *= mine[0][i];
-                            tm_st<NC>(o, tmem + tm_lane + j * N + c0);
+                                for (int i = 0; i < 8; i++) o[i] *= mine[0][h + i];
+                                tm_st<8>(o, tmem + tm_lane + j * N + c0 + h);
+                            }
                         }
                     }
                     __syncwarp();
@@ -1056,7 +1080,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 uint32_t pk[NC / 2];
 #pragma unroll
                 for (int i = 0; i < NC; i += 2) {
-                    const float e0 = ex2(y[i]), e1 = ex2(y[i + 1]);
+                    const float e0 = ex2(x[i]), e1 = ex2(x[i + 1]);
                     l[i] += e0;
                     l[i + 1] += e1;
                     pk[i / 2] = pack2<T>(e0, e1);
@@ -1071,24 +1095,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 tc_fence_before();
                 __syncwarp();                                 /* an arrival a warp: they are serial */
                 if (lane == 0) mbar_arrive(&c.p_ready);
-                slot0 += npair;
-                if (slot0 >= Cfg::pairs) { slot0 -= Cfg::pairs; par0 ^= 1; }
             }
+            pos += (g.k1 - g.k0) * npair;
             /* the next segment's queries first: its products run under what follows */
             bar_named(5, kTcSoft);
-            const bool more = c.more[cur ^ 1];
+            const bool more = c.more[then];
             if (more) {
-                tables(cur ^ 1);
+                tables(then, which ^ 1);
                 bar_named(5, kTcSoft);
-                queries(cur ^ 1);
+                queries(then);
             }
             /* ---- the segment's result ---- */
-            const int lc = lane % NC;
-            float m = kNone;
-#pragma unroll
-            for (int i = 0; i < NC; i++)
-                if (lc == i) m = ref[i];
-            float sum = lane_sums<NC>(l, lane);               /* of column c0 + lc           */
+            const int lc = min(lane, NC - 1);
+            const float m = mine[1][lc];                      /* of column c0 + lc           */
+            float sum = lane_sums<NC>(l, lane);
             if (lane < NC) sx[quad][lane] = sum;
             bar_named(1 + quarter, 128);
             sum = (sx[0][lc] + sx[1][lc]) + (sx[2][lc] + sx[3][lc]);
@@ -1124,7 +1144,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
 #pragma unroll
                         for (int i = 0; i < NC; i++)
                             if (i < nc)
-                                dst[c.ooff[cur][c0 + i]] = from_f<T>(some && mine[0][i] != 0.0f ? o[i] * mine[0][i] : 0.0f);
+                                dst[c.ooff[which][c0 + i]] = from_f<T>(some && mine[0][i] != 0.0f ? o[i] * mine[0][i] : 0.0f);
                     } else {
                         float *dst = p.part + (slot * N + c0) * p.part_ld + cd;
 #pragma unroll
@@ -1136,6 +1156,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
             tc_fence_before();
             if (st == 0) note_split(p, g, w.all);
             if (!more) break;
+            cur = then;
         }
     }
     __syncthreads();
@@ -1336,8 +1357,8 @@ cudaError_t tc_launch(Shape &p, const CUtensorMap &map, int box_rows, int sms, c
     p.KT = kTcKeys;
     p.kt_log = 7;
     carve(&p, sms);
-    const size_t smem = TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024;
-    static_assert(TcCfg<N>::off_ctl + sizeof(TcCtl) + 1024 <= 227 * 1024, "attention tile exceeds shared memory");
+    const size_t smem = TcCfg<N>::off_ctl + sizeof(TcCtl<N>) + 1024;
+    static_assert(TcCfg<N>::off_ctl + sizeof(TcCtl<N>) + 1024 <= 227 * 1024, "attention tile exceeds shared memory");
     cudaError_t e = cudaFuncSetAttribute(mla_tc_kernel<T, N, TMA>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return e;
