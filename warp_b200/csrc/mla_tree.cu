@@ -225,21 +225,23 @@ __device__ __forceinline__ void note_split(const Shape &p, const Seg &s, int all
  * fp32 arithmetic throughout. A CTA of 256 threads takes 32 query rows by
  * tiles of 32 keys, both as fp32 rows in shared memory, rows 16 bytes past a
  * multiple of 128 apart so that float4 loads of successive rows meet no bank
- * twice. Scores: two groups of four warps take half of the columns each, a
- * thread 4 rows by 2 keys (6 loads of 16 bytes for 32 FMAs), and the halves
- * are added. Products: a thread owns two of the kl columns for all rows, the
- * weights broadcast (10 loads' worth of shared memory for 64 FMAs a key).
- * So the FMA rate bounds it: 32 x 32 rows of 512 + 64 are 8.7 k cycles of
- * it. Where rows are fp32 and 16-byte aligned the next tile's are copied
- * asynchronously meanwhile, if two tiles fit. */
+ * twice. Scores and softmax: a lane has a key, a warp 4 rows, which its lanes
+ * read together; the scores never leave the registers. Products: a thread owns
+ * two of the kl columns for all rows, the weights read together (10 loads'
+ * worth of shared memory for 64 FMAs a key). Shared memory bounds the scores
+ * (32 x 32 rows of 512 + 64: 15 k cycles), the FMA rate the products (7 k). A
+ * lone token of 32 heads over 4096 rows, one tile a CTA, takes 29 us with the
+ * joining, a third of it cold starts: code that runs once is kept small.
+ * Where rows are fp32 and 16-byte aligned the next tile's are copied asynchronously
+ * meanwhile, if two tiles fit. */
 constexpr int kGenThreads = 256;
 constexpr int kGenRows = 32;
 constexpr int kGenKeys = 32;
 
 struct alignas(16) GenSmem {
-    float p[kGenKeys][kGenRows];     /* scores (key, row), then weights           */
-    float h[kGenKeys][kGenRows];     /* the second half's scores                  */
+    float p[kGenKeys][kGenRows + 4]; /* weights (key, row)                        */
     float m[kGenRows], l[kGenRows], a[kGenRows];
+    long long off[kGenRows];         /* a row's elements in o                     */
     int tok[kGenRows];               /* a row's token in the request              */
     int bad[kGenKeys];               /* a new row that holds no finite number     */
     WalkSmem walk;
@@ -326,34 +328,6 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncthreads();
             if (bufs == 2 && kt + 1 < g.k1) fetch(g, kt + 1, buf ^ 1);
-            {
-                const int half = warp >> 2, t4 = tid & 127, rg = t4 & 7, kg = t4 >> 3;   /* rows rg + 8i, keys kg + 16j */
-                float sum[4][2] = {};
-                if (rg < rows) {
-                    const float *qp = qs + rg * ld, *kp = kb + kg * ld;
-#pragma unroll 4
-                    for (int v = half; v < nv; v += 2) {
-                        float4 q[4], k[2];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) q[i] = *reinterpret_cast<const float4 *>(qp + i * 8 * ld + v * 4);
-#pragma unroll
-                        for (int j = 0; j < 2; j++) k[j] = *reinterpret_cast<const float4 *>(kp + j * 16 * ld + v * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; i++)
-#pragma unroll
-                            for (int j = 0; j < 2; j++) {
-                                sum[i][j] = fmaf(q[i].x, k[j].x, sum[i][j]);
-                                sum[i][j] = fmaf(q[i].y, k[j].y, sum[i][j]);
-                                sum[i][j] = fmaf(q[i].z, k[j].z, sum[i][j]);
-                                sum[i][j] = fmaf(q[i].w, k[j].w, sum[i][j]);
-                            }
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int j = 0; j < 2; j++) (half ? s.h : s.p)[kg + 16 * j][rg + 8 * i] = sum[i][j];
-            }
             if (tail) {
                 /* a new row that holds a NaN or an infinity is zeros to the products;
                  * who sees it gets NaN weights, who does not is not touched */
@@ -364,58 +338,72 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                     for (int i = tid & 7; i < kl; i += 8) bad |= !isfinite(row[i]);
                 bad = (__ballot_sync(0xffffffffu, bad) >> (lane & 24)) & 0xff;
                 if ((tid & 7) == 0) s.bad[k] = bad;
-                __syncthreads();                              /* the scores have read it     */
                 if (bad)
                     for (int i = tid & 7; i < kl; i += 8) row[i] = 0.0f;
+                __syncthreads();
             }
-            __syncthreads();
-            /* softmax: a key a lane, 4 rows a warp */
-#pragma unroll
-            for (int i = 0; i < kGenRows / 8; i++) {
-                const int row = warp + 8 * i, key = k0 + lane;
-                if (row >= rows) break;
-                float x = (s.p[lane][row] + s.h[lane][row]) * d.scale;
-                if (tail) {
-                    const bool see = key < g.vis && (key < g.q.ctx || sees(p, g.q, s.tok[row], key - g.q.ctx));
-                    if (!see) x = -INFINITY;
-                    else if (s.bad[lane]) x = __int_as_float(0x7fc00000);
-                }
-                float mx = x;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                const float m0 = s.m[row], m1 = fmaxf(m0, mx), ref = m1 == -INFINITY ? 0.0f : m1;
-                /* a masked key weighs exactly nothing; a NaN score stays one */
-                const float e = x == -INFINITY ? 0.0f : expf(x - ref);
-                float sum = e;
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                s.p[lane][row] = e;
-                __syncwarp();
-                if (lane == 0) {
-                    const float a = m0 == -INFINITY ? 0.0f : expf(m0 - ref);
-                    s.a[row] = a;
-                    s.l[row] = s.l[row] * a + sum;
-                    s.m[row] = m1;
-                }
-            }
-            __syncthreads();
-            const int c0 = 2 * tid;
-#pragma unroll
-            for (int i = 0; i < kGenRows / 4; i++) {
-                if (4 * i >= rows) break;
-                const float4 a = *reinterpret_cast<const float4 *>(s.a + 4 * i);
-                const float aa[4] = { a.x, a.y, a.z, a.w };
-#pragma unroll
-                for (int z = 0; z < 4; z++) { acc[0][4 * i + z] *= aa[z]; acc[1][4 * i + z] *= aa[z]; }
-            }
-            if (c0 < kl) {
+            const int r0 = 4 * warp;
+            if (r0 < rows) {
+                float x[4] = {};
+                const float4 *kp = reinterpret_cast<const float4 *>(kb + lane * ld);
+                const float4 *qp = reinterpret_cast<const float4 *>(qs + r0 * ld);
 #pragma unroll 4
+                for (int v = 0; v < nv; v++) {
+                    const float4 k = kp[v];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4 q = qp[i * (ld / 4) + v];
+                        x[i] = fmaf(q.x, k.x, x[i]);
+                        x[i] = fmaf(q.y, k.y, x[i]);
+                        x[i] = fmaf(q.z, k.z, x[i]);
+                        x[i] = fmaf(q.w, k.w, x[i]);
+                    }
+                }
+                const int key = k0 + lane;
+                float e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    x[i] *= d.scale;
+                    if (tail) {
+                        const bool see = key < g.vis && (key < g.q.ctx || (r0 + i < rows && sees(p, g.q, s.tok[r0 + i], key - g.q.ctx)));
+                        if (!see) x[i] = -INFINITY;
+                        else if (s.bad[lane]) x[i] = __int_as_float(0x7fc00000);
+                    }
+                    float mx = x[i];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                    const float m0 = s.m[r0 + i], m1 = fmaxf(m0, mx), ref = m1 == -INFINITY ? 0.0f : m1;
+                    /* a masked key weighs exactly nothing; a NaN score stays one */
+                    e[i] = x[i] == -INFINITY ? 0.0f : expf(x[i] - ref);
+                    float sum = e[i];
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    __syncwarp();
+                    if (lane == 0) {
+                        const float a = m0 == -INFINITY ? 0.0f : expf(m0 - ref);
+                        s.a[r0 + i] = a;
+                        s.l[r0 + i] = s.l[r0 + i] * a + sum;
+                        s.m[r0 + i] = m1;
+                    }
+                }
+                *reinterpret_cast<float4 *>(&s.p[lane][r0]) = make_float4(e[0], e[1], e[2], e[3]);
+            }
+            __syncthreads();
+            /* rows by 8: rows past the tile's own are not looked at */
+            auto products = [&](auto quads) {
+                constexpr int kQuads = decltype(quads)::value;
+#pragma unroll
+                for (int i = 0; i < kQuads; i++) {
+                    const float4 a = *reinterpret_cast<const float4 *>(s.a + 4 * i);
+                    acc[0][4 * i] *= a.x; acc[0][4 * i + 1] *= a.y; acc[0][4 * i + 2] *= a.z; acc[0][4 * i + 3] *= a.w;
+                    acc[1][4 * i] *= a.x; acc[1][4 * i + 1] *= a.y; acc[1][4 * i + 2] *= a.z; acc[1][4 * i + 3] *= a.w;
+                }
+#pragma unroll 2
                 for (int k = 0; k < kGenKeys; k++) {
-                    const float2 v = *reinterpret_cast<const float2 *>(kb + k * ld + c0);
+                    const float2 v = *reinterpret_cast<const float2 *>(kb + k * ld + 2 * tid);
                     const float4 *pk = reinterpret_cast<const float4 *>(s.p[k]);
 #pragma unroll
-                    for (int i = 0; i < kGenRows / 4; i++) {
-                        if (4 * i >= rows) break;
+                    for (int i = 0; i < kQuads; i++) {
                         const float4 e = pk[i];
                         const float ee[4] = { e.x, e.y, e.z, e.w };
 #pragma unroll
@@ -425,6 +413,10 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                         }
                     }
                 }
+            };
+            if (2 * tid < kl) {
+                if (rows <= 8) products(std::integral_constant<int, 2>());
+                else products(std::integral_constant<int, 8>());
             }
             if (bufs == 1 && kt + 1 < g.k1) {
                 __syncthreads();
@@ -434,19 +426,31 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
         __syncthreads();
         const bool whole = g.first && g.last;
         const int slot = part_slot(g), c0 = 2 * tid;
-#pragma unroll
-        for (int i = 0; i < kGenRows; i++) {
-            if (i >= rows) break;
-            const float l = s.l[i], inv = l == 0.0f ? 0.0f : 1.0f / l;
-            if (whole) {
-                const int tok = s.tok[i], h = g.row0 + i - tok * H;
-                T *o = static_cast<T *>(d.o) + (size_t)(g.q.q0 + tok) * d.o_token_stride + (size_t)h * d.o_head_stride;
-                if (c0 < kl) o[c0] = from_f<T>(l == 0.0f ? 0.0f : acc[0][i] * inv);
-                if (c0 + 1 < kl) o[c0 + 1] = from_f<T>(l == 0.0f ? 0.0f : acc[1][i] * inv);
-            } else {
-                float *o = p.part + ((size_t)slot * kGenRows + i) * p.part_ld;
-                if (c0 < p.part_ld) *reinterpret_cast<float2 *>(o + c0) = make_float2(acc[0][i], acc[1][i]);
+        if (whole) {
+            if (tid < kGenRows) {
+                const int tok = s.tok[tid], h = g.row0 + tid - tok * H;
+                s.a[tid] = tid < rows && s.l[tid] != 0.0f ? 1.0f / s.l[tid] : 0.0f;
+                s.off[tid] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
             }
+            __syncthreads();
+        }
+        /* little code a row: it is fetched cold, once (32 divisions and both ways of
+         * storing, unrolled, took 24 k cycles) */
+        if (whole) {
+            T *o = static_cast<T *>(d.o) + c0;
+#pragma unroll
+            for (int i = 0; i < kGenRows; i++)
+                if (i < rows && c0 < kl) {
+                    const float inv = s.a[i];
+                    T *to = o + s.off[i];
+                    to[0] = from_f<T>(inv == 0.0f ? 0.0f : acc[0][i] * inv);
+                    if (c0 + 1 < kl) to[1] = from_f<T>(inv == 0.0f ? 0.0f : acc[1][i] * inv);
+                }
+        } else if (c0 < p.part_ld) {
+            float *o = p.part + (size_t)slot * kGenRows * p.part_ld + c0;
+#pragma unroll
+            for (int i = 0; i < kGenRows; i++)
+                if (i < rows) *reinterpret_cast<float2 *>(o + i * p.part_ld) = make_float2(acc[0][i], acc[1][i]);
         }
         if (tid < rows) {
             const float m = s.m[tid], l = s.l[tid];
