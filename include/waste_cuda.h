@@ -402,6 +402,8 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
 #define WASTE_CUDA_DERR_BAD_TREE  32u  /* kv_plan: a parent that is no earlier node (taken as a
                                            root), a tree of more than 32 * mask_words nodes (not
                                            served), or more new tokens than T (left out) */
+#define WASTE_CUDA_DERR_BAD_MASK  64u  /* logits_adjust: a row's mask number is not below
+                                           n_allow; the row was left without a mask */
 unsigned waste_cuda_device_errors(void);
 
 /* ---- single VQ3R kernels ---------------------------------------------------
@@ -654,7 +656,8 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  * default stream. The calling thread's current device must be the one the
  * library is bound to. Lengths, ids and tables are read on the device
  * only; a value out of range there never moves an access outside the
- * caller's buffers: it raises a bit of waste_cuda_device_errors.
+ * caller's buffers: it raises a bit of waste_cuda_device_errors. A captured
+ * graph is valid until waste_cuda_shutdown.
  *
  * A new token t of request r is row t of the step's arrays, with
  * q_indptr[r] <= t < q_indptr[r+1]. Its latent lies in the cache at the
@@ -737,7 +740,7 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * [T][heads][kl] and q [T][heads][kl + rope] at the given strides in
  * elements; rows behind q_indptr[B] are left as they are. kl 1..512, rope
  * 0..128, page >= 1, mask_words * 32 >= the most new tokens of a request.
- * n_blocks: blocks in the cache. ws: waste_cuda_mla_tree_ws_bytes(heads,
+ * n_blocks: blocks in the cache. o overlaps no input. ws: waste_cuda_mla_tree_ws_bytes(heads,
  * kl) bytes on the device, 256-byte aligned, not shared by calls that may
  * overlap (another stream, another captured graph); nothing in it has to
  * be set, or survives the call. Results do not depend on what runs beside
@@ -774,7 +777,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  * and produced for that row. bias_id / bias_val: request r's entries are
  * bias_indptr[r] .. bias_indptr[r+1] (NULL: none). allow
  * [n_allow][allow_words] bits (NULL: none): row t is under mask
- * allow_row[t], or under none if that is negative; allow_row NULL: mask t.
+ * allow_row[t], or under none if that is negative (a number that is not
+ * below n_allow raises BAD_MASK); allow_row NULL: mask t.
  * rep, freq, pres, hist NULL: 1, 0, 0, empty. Ids outside 0..V-1 are
  * ignored. ld, ld_out: elements between rows; out may be logits with the
  * same ld. Rows behind q_indptr[B] are left as they are. B up to 4096, R up

@@ -112,12 +112,15 @@ def attn(q, cache, table, kv_len, indptr, mask, scale, kl, page, dtype):
     return o, lse, to, tl
 
 
-def logits(x, indptr, hist, hist_len, prompt_len, rep, freq, pres, draft, tree, bias, allow, allow_row):
-    """One row at a time: x [R][V] (64 bits); bias: per request a list of (id, value)."""
+def logits(x, indptr, hist, hist_len, prompt_len, rep, freq, pres, draft, tree, bias, allow, allow_row, only=None):
+    """One row at a time: x [R][V] (64 bits); bias: per request a list of (id, value);
+    only: the rows to do."""
     R, V = x.shape
     out = x.clone()
     for r in range(len(indptr) - 1):
         for t in range(indptr[r], indptr[r + 1]):
+            if only is not None and t not in only:
+                continue
             seen, n = torch.zeros(V, dtype=torch.bool), torch.zeros(V, dtype=torch.float64)
             if hist is not None:
                 for i, v in enumerate(hist[r][:hist_len[r]]):

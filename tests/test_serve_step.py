@@ -41,7 +41,7 @@ def tree(**kw):
 def logits(**kw):
     p = {n: A + 64 * i for i, (n, t) in enumerate(wb.LogitsAdjust._fields_) if t is C.c_void_p}
     return wb.LogitsAdjust(**{**dict(B=2, R=4, V=1000, dtype=0, tree_words=1, allow_words=32, n_allow=4,
-                                     hist_stride=16, ld=1000, ld_out=1000), **p, **kw})
+                                     hist_stride=16, ld=1000, ld_out=1000), **p, "out": A + (1 << 16), **kw})
 
 
 REFUSED = [
@@ -52,6 +52,8 @@ REFUSED = [
     ("kv_plan_dev", plan, dict(slot=None)), ("kv_plan_dev", plan, dict(short_blocks=None)),
     ("kv_plan_dev", plan, dict(mask=None)), ("kv_plan_dev", plan, dict(mask_words=0)),
     ("kv_plan_dev", plan, dict(kv_len=A, ctx_len=A)), ("kv_plan_dev", plan, dict(slot=A + 4)),
+    ("kv_plan_dev", plan, dict(n_blocks=A, n_blocks_out=A + 4)), ("kv_plan_dev", plan, dict(n_blocks=A, kv_len=A)),
+    ("kv_plan_dev", plan, dict(q_len=A + 8, q_indptr=A)),
     ("mla_rows_dev", rows, dict(T=-1)), ("mla_rows_dev", rows, dict(kl=0)), ("mla_rows_dev", rows, dict(kl=4097)),
     ("mla_rows_dev", rows, dict(rope=63)), ("mla_rows_dev", rows, dict(rope=514)),
     ("mla_rows_dev", rows, dict(dtype=3)), ("mla_rows_dev", rows, dict(x_dtype=-1)),
@@ -66,7 +68,9 @@ REFUSED = [
     ("mla_tree_attn_dev", tree, dict(scale=float("inf"))), ("mla_tree_attn_dev", tree, dict(scale=float("nan"))),
     ("mla_tree_attn_dev", tree, dict(mask_words=0)), ("mla_tree_attn_dev", tree, dict(ws=A + 16)),
     ("mla_tree_attn_dev", tree, dict(q=None)), ("mla_tree_attn_dev", tree, dict(o=A + 1)),
-    ("logits_adjust_dev", logits, dict(V=0)), ("logits_adjust_dev", logits, dict(B=65536)),
+    ("mla_tree_attn_dev", tree, dict(o=A, q=A)),
+    ("logits_adjust_dev", logits, dict(V=0)), ("logits_adjust_dev", logits, dict(B=4097)),
+    ("logits_adjust_dev", logits, dict(R=65536)), ("logits_adjust_dev", logits, dict(logits=A, out=A + 400)),
     ("logits_adjust_dev", logits, dict(ld=999)), ("logits_adjust_dev", logits, dict(ld_out=999)),
     ("logits_adjust_dev", logits, dict(dtype=3)), ("logits_adjust_dev", logits, dict(q_indptr=None)),
     ("logits_adjust_dev", logits, dict(hist_len=None)), ("logits_adjust_dev", logits, dict(draft=None)),

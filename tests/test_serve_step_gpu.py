@@ -453,6 +453,37 @@ def test_attn_extreme_scores(cuda_lib, name):
     a.call().check()
 
 
+@pytest.mark.parametrize("name", ["tree", "many_singles", "f32_tree"])
+def test_attn_scale_zero(cuda_lib, name):
+    """All seen rows weigh the same; masked ones nothing."""
+    a = attn_case(cuda_lib, name)
+    a.scale = 0.0
+    a.put().call().check()
+
+
+def test_attn_two_threads(cuda_lib):
+    """Calls from two host threads, each on its stream with its workspace."""
+    import threading
+    cases = [attn_case(cuda_lib, "many_pairs").put(), attn_case(cuda_lib, "many_singles").put()]
+    refs = [c.ref() for c in cases]
+
+    def run(c):
+        torch.cuda.set_device(0)
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                c.call()
+            torch.cuda.current_stream().synchronize()
+
+    torch.cuda.synchronize()
+    ts = [threading.Thread(target=run, args=(c,)) for c in cases]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    for c, ref in zip(cases, refs):
+        c.check(ref)
+
+
 def test_attn_nan_query(cuda_lib):
     """A NaN in one query row stays in its row."""
     for name in ("tree", "f32_tree"):
@@ -668,6 +699,44 @@ def test_logits_parts(cuda_lib, use, inplace):
             setattr(c.d, k, None)
     cuda_lib.logits_adjust_dev(c.d, stream())
     c.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logits_many_named(cuda_lib, dtype):
+    """More named ids in a slice than are taken at once, and more drafted ones
+    than are listed."""
+    c = Logits(cuda_lib, 12, dtype, 30000, [1, 300], 9000, 700)
+    rng = random.Random(1)
+    for r in range(2):
+        c.hist[r] = rng.sample(range(30000), 9000)
+        c.hist_len[r], c.prompt_len[r] = 9000, 4000
+    c.draft[1:] = [rng.randrange(2000) for _ in range(300)]
+    for k in ("hist", "hist_len", "prompt_len", "draft"):
+        c.t[k].copy_(dev(getattr(c, k)).view(c.t[k].shape))
+    cuda_lib.logits_adjust_dev(c.d, stream())
+    rows = [0, 1, 2, 150, 300]
+    got = c.gy.clone()
+    torch.cuda.synchronize()
+    # the definition goes row by row: a few of the rows
+    x = c.x[:c.R, :c.V].double()
+    ref = O.logits(x, c.indptr, c.hist, c.hist_len, c.prompt_len, c.rep, c.freq, c.pres, c.draft, c.tree, c.bias, c.allow,
+                   c.allow_row, only=rows)
+    for t in rows:
+        fin = ~torch.isinf(ref[t])
+        g = got[t, :c.V].cpu().double()
+        assert torch.equal(torch.isinf(g), ~fin)
+        size = x[t].abs() * 1.5 + 0.5 * 310 + 0.6 + 12
+        tol = ref[t].abs() * HALF[dtype] + 8 * E * size + TINY[dtype]
+        assert bool(((g - ref[t]).abs() <= tol)[fin].all())
+
+
+def test_logits_mask_out_of_range(cuda_lib):
+    wb = cuda_lib
+    c = Logits(wb, 3, "f32", 500, [1, 1], 4, 2, use=("allow", "rows"), extra=0)
+    c.t["allow_row"].copy_(dev([c.d.n_allow, 0]))
+    wb.logits_adjust_dev(c.d, stream())
+    assert wb.device_errors() == wb.DERR_BAD_MASK
+    assert bool(torch.isfinite(c.gy[0]).all()) and bool(torch.isinf(c.gy[1]).all())
 
 
 def test_logits_row_per_request(cuda_lib):

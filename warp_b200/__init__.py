@@ -51,7 +51,7 @@ PHASES = ("router", "act", "gateup", "down", "combine", "matvec", "matvec_reduce
 
 OK, E_ARG, E_DEVICE, E_RECORD, E_NOBANK, E_NOMEM, E_NODEV = 0, -1, -2, -3, -4, -5, -6
 DERR_ROUTE_WAIT, DERR_TMA_WAIT, DERR_BAD_EXPERT, DERR_PEER_WAIT = 1, 2, 4, 8
-DERR_BAD_BLOCK, DERR_BAD_TREE = 16, 32
+DERR_BAD_BLOCK, DERR_BAD_TREE, DERR_BAD_MASK = 16, 32, 64
 F32, F16, BF16 = 0, 1, 2
 
 

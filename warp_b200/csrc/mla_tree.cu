@@ -527,6 +527,7 @@ template <int N> struct TcCtl {
     /* the softmax warps' segments: the next is found while some are at the last */
     Seg seg[3];
     int more[3];
+    Walk walk_soft;                  /* theirs: the other roles may still read walk's */
 };
 
 template <int N>
@@ -946,14 +947,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
             if (lane == 0) mbar_arrive(&c.q_full);
         };
         auto next = [&](int i) {                              /* one thread                  */
-            Walk v = c.walk.w;
+            Walk v = c.walk_soft;
             Seg n;
             c.more[i] = walk_next(p, v, n);
-            c.walk.w = v;
+            c.walk_soft = v;
             c.seg[i] = n;
         };
-        bar_named(5, kTcSoft);                                /* every role has the start    */
-        if (st == 0) next(0);
+        if (st == 0) {
+            c.walk_soft = w;
+            next(0);
+        }
         bar_named(5, kTcSoft);
         tables(0, 0);
         bar_named(5, kTcSoft);

@@ -346,7 +346,8 @@ template <typename T> __device__ __forceinline__ void mask_vec(uint4 &v, uint32_
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda_logits_desc d, int vs)
+__global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda_logits_desc d, int vs,
+                                                                unsigned int *err)
 {
     constexpr int E = 16 / sizeof(T), U = 8;
     extern __shared__ __align__(16) unsigned char sml[];
@@ -397,6 +398,7 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     if (tid < rows) {
         const int a = !d.allow ? -1 : d.allow_row ? d.allow_row[t0 + tid] : t0 + tid;
         s.mask[tid] = a < d.n_allow ? a : -1;
+        if (d.allow && a >= d.n_allow) atomicOr(err, WASTE_CUDA_DERR_BAD_MASK);
     }
     if (ht >= 0) {
 #pragma unroll
@@ -616,7 +618,7 @@ cudaError_t rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, cu
 }
 
 template <typename T>
-cudaError_t logits_launch(const waste_cuda_logits_desc *d, int sms, cudaStream_t s)
+cudaError_t logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, int sms, cudaStream_t s)
 {
     /* as many slices as are resident at once, two CTAs an SM: a few more wait for
      * a whole turn, fewer read the history less often */
@@ -631,7 +633,7 @@ cudaError_t logits_launch(const waste_cuda_logits_desc *d, int sms, cudaStream_t
     cudaError_t e = cudaFuncSetAttribute(logits_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)sizeof(LogitSmem));
     if (e != cudaSuccess) return e;
-    logits_kernel<T><<<dim3((d->V + vs - 1) / vs, chunks), kLogThreads, sizeof(LogitSmem), s>>>(*d, vs);
+    logits_kernel<T><<<dim3((d->V + vs - 1) / vs, chunks), kLogThreads, sizeof(LogitSmem), s>>>(*d, vs, err);
     return cudaGetLastError();
 }
 
@@ -682,13 +684,13 @@ int wc_mla_rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, voi
     return (int)rows_launch<__nv_bfloat16>(d, err, s);
 }
 
-int wc_logits_launch(const waste_cuda_logits_desc *d, int sms, void *stream)
+int wc_logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, int sms, void *stream)
 {
     const cudaStream_t s = (cudaStream_t)stream;
     wc_count_launches(1);
-    if (d->dtype == WASTE_CUDA_F32) return (int)logits_launch<float>(d, sms, s);
-    if (d->dtype == WASTE_CUDA_F16) return (int)logits_launch<__half>(d, sms, s);
-    return (int)logits_launch<__nv_bfloat16>(d, sms, s);
+    if (d->dtype == WASTE_CUDA_F32) return (int)logits_launch<float>(d, err, sms, s);
+    if (d->dtype == WASTE_CUDA_F16) return (int)logits_launch<__half>(d, err, sms, s);
+    return (int)logits_launch<__nv_bfloat16>(d, err, sms, s);
 }
 
 } /* extern "C" */

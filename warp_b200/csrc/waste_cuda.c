@@ -3307,6 +3307,12 @@ static size_t dtype_size(int dtype)
 
 static int misaligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 
+/* n bytes at a and m at b share some */
+static int overlap(const void *a, size_t n, const void *b, size_t m)
+{
+    return (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
+}
+
 /* The caller holds g_mu: the library is bound and its device is current. */
 static int serve_ready(const char *what)
 {
@@ -3329,10 +3335,16 @@ int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream)
         return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: bad sizes or a missing array (B 1..4096)");
     if ((d->mask && d->mask_words < 1) || (d->parent && !d->mask))
         return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: a tree needs a mask of mask_words >= 1");
-    if (d->kv_len == d->ctx_len || d->kv_len == d->q_len || d->q_indptr == d->ctx_len ||
-        d->q_indptr == d->q_len || d->n_blocks_out == d->ctx_len || d->n_blocks_out == d->q_len ||
-        d->n_blocks_out == d->kv_len || misaligned(d->slot, 8))
-        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: only the counts may be updated in place");
+    const size_t nb = (size_t)d->B * sizeof(int);
+    int *const outs[3] = { d->kv_len, d->q_indptr, d->n_blocks_out };
+    for (int k = 0; k < 3; k++) {
+        const size_t n = k == 1 ? nb + sizeof(int) : nb;
+        if (overlap(outs[k], n, d->ctx_len, nb) || overlap(outs[k], n, d->q_len, nb) ||
+            (overlap(outs[k], n, d->n_blocks, nb) && outs[k] != d->n_blocks) ||
+            (k < 2 && outs[k] == d->n_blocks))
+            return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: only the counts may be updated in place");
+    }
+    if (misaligned(d->slot, 8)) return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: slot is not 8-byte aligned");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("kv_plan_dev"))) goto out;
     CK((cudaError_t)wc_kv_plan_launch(d, S.d_serr, stream ? stream : (void *)S.stream), "kv_plan");
@@ -3385,7 +3397,7 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
     const size_t z = dtype_size(d->dtype);
     if (!d->q || !d->cache || !d->block_table || !d->kv_len || !d->q_indptr || !d->o || !d->ws ||
         (d->mask && d->mask_words < 1) || misaligned(d->q, z) || misaligned(d->cache, z) ||
-        misaligned(d->o, z) || misaligned(d->ws, 256))
+        misaligned(d->o, z) || misaligned(d->ws, 256) || d->o == d->q || d->o == d->cache)
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("mla_tree_attn_dev"))) goto out;
@@ -3442,9 +3454,13 @@ int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream)
         (d->allow && ((int64_t)d->allow_words * 32 < d->V || d->n_allow < 0)) ||
         misaligned(d->logits, dtype_size(d->dtype)) || misaligned(d->out, dtype_size(d->dtype)))
         return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: a missing, short or misaligned array");
+    const size_t z = dtype_size(d->dtype);
+    if (d->out != d->logits && overlap(d->out, ((size_t)(d->R - 1) * d->ld_out + d->V) * z, d->logits,
+                                       ((size_t)(d->R - 1) * d->ld + d->V) * z))
+        return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: out overlaps logits and is not the same");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("logits_adjust_dev"))) goto out;
-    CK((cudaError_t)wc_logits_launch(d, S.sms, stream ? stream : (void *)S.stream),
+    CK((cudaError_t)wc_logits_launch(d, S.d_serr, S.sms, stream ? stream : (void *)S.stream),
        "logits_adjust");
 out:
     pthread_mutex_unlock(&g_mu);

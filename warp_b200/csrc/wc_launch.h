@@ -370,7 +370,8 @@ int    wc_mla_tree_box(const waste_cuda_mla_tree_desc *d);
  * 128 bytes. */
 int    wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *map, int box_rows,
                           unsigned int *err, int sms, void *stream);
-int    wc_logits_launch(const waste_cuda_logits_desc *d, int sms, void *stream);
+int    wc_logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, int sms,
+                        void *stream);
 
 /* Phase timers (see waste_cuda_profile in include/waste_cuda.h). */
 enum { WC_PH_ROUTER, WC_PH_ACT, WC_PH_GATEUP, WC_PH_DOWN, WC_PH_COMBINE,
