@@ -318,6 +318,10 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                 for (int j = tid & 7; j < D; j += 8) qs[i * ld + j] = i < rows ? to_f(src[j]) : 0.0f;
             }
         }
+        /* the products' threads: two columns each, and where kl leaves threads over,
+         * a part of the rows (in quads from quad0) */
+        const int ct = kl > 256 ? 256 : kl > 128 ? 128 : kl > 64 ? 64 : 32, nq = kGenRows / 4 * ct / kGenThreads;
+        const int c0 = 2 * (tid % ct), quad0 = tid / ct * nq;
         float acc[2][kGenRows];
 #pragma unroll
         for (int i = 0; i < kGenRows; i++) acc[0][i] = acc[1][i] = 0.0f;
@@ -344,7 +348,7 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             }
             const int r0 = 4 * warp;
             if (r0 < rows) {
-                float x[4] = {};
+                float4 sum[4] = {};                           /* four chains a row           */
                 const float4 *kp = reinterpret_cast<const float4 *>(kb + lane * ld);
                 const float4 *qp = reinterpret_cast<const float4 *>(qs + r0 * ld);
 #pragma unroll 4
@@ -353,28 +357,28 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float4 q = qp[i * (ld / 4) + v];
-                        x[i] = fmaf(q.x, k.x, x[i]);
-                        x[i] = fmaf(q.y, k.y, x[i]);
-                        x[i] = fmaf(q.z, k.z, x[i]);
-                        x[i] = fmaf(q.w, k.w, x[i]);
+                        sum[i].x = fmaf(q.x, k.x, sum[i].x);
+                        sum[i].y = fmaf(q.y, k.y, sum[i].y);
+                        sum[i].z = fmaf(q.z, k.z, sum[i].z);
+                        sum[i].w = fmaf(q.w, k.w, sum[i].w);
                     }
                 }
                 const int key = k0 + lane;
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    x[i] *= d.scale;
+                    float x = ((sum[i].x + sum[i].y) + (sum[i].z + sum[i].w)) * d.scale;
                     if (tail) {
                         const bool see = key < g.vis && (key < g.q.ctx || (r0 + i < rows && sees(p, g.q, s.tok[r0 + i], key - g.q.ctx)));
-                        if (!see) x[i] = -INFINITY;
-                        else if (s.bad[lane]) x[i] = __int_as_float(0x7fc00000);
+                        if (!see) x = -INFINITY;
+                        else if (s.bad[lane]) x = __int_as_float(0x7fc00000);
                     }
-                    float mx = x[i];
+                    float mx = x;
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
                     const float m0 = s.m[r0 + i], m1 = fmaxf(m0, mx), ref = m1 == -INFINITY ? 0.0f : m1;
                     /* a masked key weighs exactly nothing; a NaN score stays one */
-                    e[i] = x[i] == -INFINITY ? 0.0f : expf(x[i] - ref);
+                    e[i] = x == -INFINITY ? 0.0f : expf(x - ref);
                     float sum = e[i];
 #pragma unroll
                     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -394,14 +398,14 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                 constexpr int kQuads = decltype(quads)::value;
 #pragma unroll
                 for (int i = 0; i < kQuads; i++) {
-                    const float4 a = *reinterpret_cast<const float4 *>(s.a + 4 * i);
+                    const float4 a = *reinterpret_cast<const float4 *>(s.a + 4 * (quad0 + i));
                     acc[0][4 * i] *= a.x; acc[0][4 * i + 1] *= a.y; acc[0][4 * i + 2] *= a.z; acc[0][4 * i + 3] *= a.w;
                     acc[1][4 * i] *= a.x; acc[1][4 * i + 1] *= a.y; acc[1][4 * i + 2] *= a.z; acc[1][4 * i + 3] *= a.w;
                 }
 #pragma unroll 2
                 for (int k = 0; k < kGenKeys; k++) {
-                    const float2 v = *reinterpret_cast<const float2 *>(kb + k * ld + 2 * tid);
-                    const float4 *pk = reinterpret_cast<const float4 *>(s.p[k]);
+                    const float2 v = *reinterpret_cast<const float2 *>(kb + k * ld + c0);
+                    const float4 *pk = reinterpret_cast<const float4 *>(s.p[k]) + quad0;
 #pragma unroll
                     for (int i = 0; i < kQuads; i++) {
                         const float4 e = pk[i];
@@ -414,9 +418,11 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
                     }
                 }
             };
-            if (2 * tid < kl) {
-                if (rows <= 8) products(std::integral_constant<int, 2>());
-                else products(std::integral_constant<int, 8>());
+            if (c0 < kl && 4 * quad0 < rows) {
+                if (nq == 8 && rows > 8) products(std::integral_constant<int, 8>());
+                else if (nq == 4) products(std::integral_constant<int, 4>());
+                else if (nq == 1) products(std::integral_constant<int, 1>());
+                else products(std::integral_constant<int, 2>());
             }
             if (bufs == 1 && kt + 1 < g.k1) {
                 __syncthreads();
@@ -425,7 +431,7 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
         }
         __syncthreads();
         const bool whole = g.first && g.last;
-        const int slot = part_slot(g), c0 = 2 * tid;
+        const int slot = part_slot(g), mine = min(rows - 4 * quad0, 4 * nq);      /* rows of this thread */
         if (whole) {
             if (tid < kGenRows) {
                 const int tok = s.tok[tid], h = g.row0 + tid - tok * H;
@@ -440,17 +446,17 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             T *o = static_cast<T *>(d.o) + c0;
 #pragma unroll
             for (int i = 0; i < kGenRows; i++)
-                if (i < rows && c0 < kl) {
-                    const float inv = s.a[i];
-                    T *to = o + s.off[i];
+                if (i < mine && c0 < kl) {
+                    const float inv = s.a[4 * quad0 + i];
+                    T *to = o + s.off[4 * quad0 + i];
                     to[0] = from_f<T>(inv == 0.0f ? 0.0f : acc[0][i] * inv);
                     if (c0 + 1 < kl) to[1] = from_f<T>(inv == 0.0f ? 0.0f : acc[1][i] * inv);
                 }
         } else if (c0 < p.part_ld) {
-            float *o = p.part + (size_t)slot * kGenRows * p.part_ld + c0;
+            float *o = p.part + ((size_t)slot * kGenRows + 4 * quad0) * p.part_ld + c0;
 #pragma unroll
             for (int i = 0; i < kGenRows; i++)
-                if (i < rows) *reinterpret_cast<float2 *>(o + i * p.part_ld) = make_float2(acc[0][i], acc[1][i]);
+                if (i < mine) *reinterpret_cast<float2 *>(o + i * p.part_ld) = make_float2(acc[0][i], acc[1][i]);
         }
         if (tid < rows) {
             const float m = s.m[tid], l = s.l[tid];
