@@ -999,15 +999,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     if (quarter == 0) c.nan_row[key_row] = 0;
                     bar_named(5, kTcSoft);
                     if (quarter < npair && key >= g.q.ctx && key < g.vis) {
-                        bool found = false;
+                        /* an exponent of ones carries into its half's top bit */
+                        constexpr uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u, one = kF16 ? 0x04000400u : 0x00800080u;
+                        uint32_t found = 0;
+#pragma unroll 4
                         for (int u = 0; u < units; u++) {
                             const uint4 v = *reinterpret_cast<const uint4 *>(
                                 mem + (u >> 3) * kTcKeys * 128 + (((u + key_row) & 7) << 4));
-                            const uint32_t e = kF16 ? 0x7c007c00u : 0x7f807f80u;
-                            found |= __vcmpeq2(v.x & e, e) || __vcmpeq2(v.y & e, e) || __vcmpeq2(v.z & e, e) ||
-                                     __vcmpeq2(v.w & e, e);
+                            found |= ((v.x & e) + one) | ((v.y & e) + one) | ((v.z & e) + one) | ((v.w & e) + one);
                         }
-                        if (found) c.nan_row[key_row] = 1;
+                        if (found & 0x80008000u) c.nan_row[key_row] = 1;
                     }
                     bar_named(5, kTcSoft);
                     bad = c.nan_row[key_row];
