@@ -38,7 +38,8 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
  * keeps them in shared memory, and takes its share of the tokens and table
  * entries. Where the counts are updated in place the CTAs are one cluster (at
  * most 8): its barrier stands between the last read of an input and the first
- * write. Which slot a token gets follows from
+ * write. 64 requests of one token take 7.3 us a call from the host, 256 trees of
+ * up to 31 nodes 8.2. Which slot a token gets follows from
  * the old table (blocks held) or the free list (blocks taken now), so no
  * table entry written here is read here. */
 constexpr int kPlanThreads = 512;
