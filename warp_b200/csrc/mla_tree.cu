@@ -498,17 +498,18 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  * times after, are the tile's maxima found (redux over the lanes, shared
  * memory over the 4 warps), the reference moved and O in TMEM rescaled.
  *
- * What bounds it. N = 32, HBM: 64 tokens over 183 k bf16 rows (216 MB) take 62
- * us, 3.5 TB/s; a tile takes 7 k cycles where its 147 KB at an SM's share of
- * HBM would take 6.4 k, and the start (lengths, table, first tile: three loads
- * one after the other), the end and the joining take a third of the time. N =
+ * What bounds it. N = 32: 64 tokens over 183 k bf16 rows (216 MB) take 60 us
+ * with the joining, 3.6 TB/s. Traced tiles took 6.7 to 7.5 k cycles, where
+ * 147 KB at an SM's share of HBM would take 6.4 k. At some ten tiles a CTA that
+ * accounts for 36 us or so; the start (lengths, table, first tile: loads that
+ * wait for one another), the end and the joining are left with the rest. N =
  * 64, the chain of a tile in one SM's shared memory: a tile is loaded (from L2:
  * 2.5 k cycles at 64 rows a box, 3.4 k at 32), its scores (36 products of 48
  * cycles, under the loads), the softmax 1.5 k, the second product 1.6 k. 512
  * tokens of 32 heads over 8192 rows take 429 us, 702 TFLOP/s; trees of 16 nodes
  * for 16 requests 108 us. Measured and slower: V loaded again instead of held,
- * for an N of 96 (554 us; two 32 KB slots do not cover L2's latency), rows sent
- * for towards L2 two tiles ahead (decode 62 -> 70 us).
+ * for an N of 96 (554 us where N = 64 took 445), rows sent for towards L2 two
+ * tiles ahead (64 tokens: 62 -> 70 us).
  *
  * Every wait is bounded: one that runs out raises WC_ERR_TMA_WAIT and
  * `dead`, upon which the roles run out their loops without waiting, issue
