@@ -599,6 +599,26 @@ def test_attn_library_stream(cuda_lib):
     a.check()
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("dtype,H,ctx", [("bf16", 32, 0), ("bf16", 32, 199), ("f16", 32, 0), ("f16", 64, 199),
+                                         ("f32", 4, 0), ("f32", 4, 99)])
+def test_attn_far_scores(cuda_lib, dtype, H, ctx, sign):
+    """Scores far beyond what 32 bits resolve to a unit, of both signs. All rows
+    seen are the same, so whatever the weights round to, o is that row: in 16
+    bits exactly, since 200 sums' 2^-24 each are no half step of the type."""
+    a = Attn(cuda_lib, 3, dtype, H, 512, 64, 64, [ctx], [1], None)
+    big = 3e4 if dtype == "f16" else 1e17
+    a.q[:] = big
+    a.cache[:] = sign * big
+    a.put().call()
+    torch.cuda.synchronize()
+    want = float(a.cache[0, 0, 0])
+    assert bool(((a.go[0].double() - want).abs() <= (512 * E * abs(want) if dtype == "f32" else 0)).all())
+    lse = float(a.q[0, 0, 0].double()) * want * 576 * a.scale
+    assert bool(((a.gl[0].double() - lse).abs() <= 700 * E * abs(lse)).all())
+    assert cuda_lib.device_errors() == 0
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

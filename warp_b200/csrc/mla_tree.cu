@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
         __syncwarp();
     } else if (any && warp >= 2) {
         /* ---- softmax ---- */
-        constexpr float kNone = -1e30f;                       /* no reference yet            */
+        constexpr float kNone = -3e38f;                       /* no reference yet            */
         const int st = tid - 64, quarter = st >> 7, quad = warp & 3, key_row = quad * 32 + lane, c0 = quarter * NC;
         const uint32_t tm_lane = (uint32_t)(quad * 32) << 16;
         const float scale2 = d.scale * 1.4426950408889634f;
@@ -1045,15 +1045,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                         if (see) seen |= 1u << i;
                     }
                 }
-                /* the exponents: x becomes x * scale2 - reference, masked ones -infinity */
+                /* the exponents: x becomes x * scale2 - reference, masked ones -infinity.
+                 * The product is rounded as the reference's was, so that the largest key's
+                 * difference is 0 at any size of the scores; fused, the product's own
+                 * rounding would be left, which at scores of 2^31 is a weight of 0 or
+                 * infinity. */
                 auto exponents = [&]() {
 #pragma unroll
                     for (int i = 0; i < NC; i += 4) {
                         const float4 r = *reinterpret_cast<const float4 *>(&mine[1][i]);
-                        x[i] = fmaf(x[i], scale2, -r.x);
-                        x[i + 1] = fmaf(x[i + 1], scale2, -r.y);
-                        x[i + 2] = fmaf(x[i + 2], scale2, -r.z);
-                        x[i + 3] = fmaf(x[i + 3], scale2, -r.w);
+                        x[i] = __fadd_rn(__fmul_rn(x[i], scale2), -r.x);
+                        x[i + 1] = __fadd_rn(__fmul_rn(x[i + 1], scale2), -r.y);
+                        x[i + 2] = __fadd_rn(__fmul_rn(x[i + 2], scale2), -r.z);
+                        x[i + 3] = __fadd_rn(__fmul_rn(x[i + 3], scale2), -r.w);
                     }
                     if (tail) {
 #pragma unroll
@@ -1070,7 +1074,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     float mx = -INFINITY;                     /* of column c0 + lane         */
 #pragma unroll
                     for (int i = 0; i < NC; i++) {
-                        const float m = warp_max(seen >> i & 1 ? x[i] * scale2 : -INFINITY);
+                        const float m = warp_max(seen >> i & 1 ? __fmul_rn(x[i], scale2) : -INFINITY);
                         if (lane == i) mx = m;
                     }
                     const int lc = min(lane, NC - 1);
