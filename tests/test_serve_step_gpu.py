@@ -619,6 +619,19 @@ def test_attn_far_scores(cuda_lib, dtype, H, ctx, sign):
     assert cuda_lib.device_errors() == 0
 
 
+@pytest.mark.parametrize("name", ["tree", "f32_tree", "pages_5"])
+def test_attn_decreasing_indptr(cuda_lib, name):
+    """Token ranges that go backwards would overlap: reported, nothing written."""
+    wb = cuda_lib
+    a = attn_case(wb, name).put()
+    ip = [0, 1] * len(a.kv)
+    a.gi.copy_(dev(ip[:len(a.kv) + 1][::-1] if len(a.kv) % 2 else ip[:len(a.kv) + 1]))
+    a.gi[0], a.gi[1] = 2, 1
+    a.call()
+    assert wb.device_errors() == wb.DERR_BAD_BLOCK
+    assert bool((a.go == 7).all()) and bool((a.gl == 7).all())
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:
