@@ -684,7 +684,7 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  *              its input's array
  *   block_table   the new entries are written, the others left as they are
  *   q_indptr [B+1], kv_len [B] (rows with the new ones), pos [T] (rotary
- *   position: ctx + depth), slot [T] (cache row), mask [T][mask_words]
+ *   position: ctx + depth; ctx for nodes past 32 * mask_words), slot [T] (cache row), mask [T][mask_words]
  *   (bit j: node j is an ancestor or the node itself; NULL allowed with a
  *   chain), short_blocks [1] (blocks that lacked, 0 if none).
  * T: rows of the per-token arrays; rows behind the last request's are left

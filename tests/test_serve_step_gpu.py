@@ -177,6 +177,18 @@ def test_plan_reports(cuda_lib):
     assert pl.t["q_indptr"].tolist() == [0, 3, 4] and pl.t["slot"].tolist() == [20, 21, 22, 24]
 
 
+def test_plan_tree_too_large(cuda_lib):
+    """A chain of nodes far past the mask's words: reported and not served, and
+    the nodes without a bit are not walked up from (their pos is the request's
+    length)."""
+    wb = cuda_lib
+    pl = Plan(wb, [5], [100], [2], np.full((1, 40), -1), list(range(50)), 0, 4, 1, [i - 1 for i in range(100)], extra=0)
+    wb.kv_plan_dev(pl.d, stream())
+    assert wb.device_errors() == wb.DERR_BAD_TREE
+    assert pl.t["kv_len"].tolist() == [0] and pl.t["slot"].tolist() == [-1] * 100
+    assert pl.t["pos"].tolist() == [5 + i for i in range(32)] + [5] * 68
+
+
 # ---- rows ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])

@@ -175,6 +175,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(
                     while (w > (j >> 5)) { row[w--] = bits; bits = 0; }
                     bits |= 1u << (j & 31);
                 }
+                /* a tree too large for its mask is not served: no walk from its far nodes,
+                 * whose length only T would bound */
+                if (!fits) break;
                 const int p = d.parent[s.qstart[r] + j];
                 if (p < 0 || p >= j) {
                     if (p != -1) bad |= WASTE_CUDA_DERR_BAD_TREE;
