@@ -401,7 +401,8 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
                                            results are not valid, nothing outside was touched */
 #define WASTE_CUDA_DERR_BAD_TREE  32u  /* kv_plan: a parent that is no earlier node (taken as a
                                            root), a tree of more than 32 * mask_words nodes (not
-                                           served), or more new tokens than T (left out) */
+                                           served), or more new tokens than T (left out);
+                                           logits_adjust: more than 4096 rows with drafts */
 #define WASTE_CUDA_DERR_BAD_MASK  64u  /* logits_adjust: a row's mask number is not below
                                            n_allow; the row was left without a mask */
 unsigned waste_cuda_device_errors(void);
@@ -775,7 +776,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  * those from prompt_len[r] on. draft [R] (NULL: none): the row's node's
  * drafted token; the tokens of the node and its ancestors (bits of
  * tree[t], tree_words words; NULL: the rows up to its own) count as seen
- * and produced for that row. bias_id / bias_val: request r's entries are
+ * and produced for that row (a request of more than 4096 rows: BAD_TREE, and
+ * its rows are as without drafts). bias_id / bias_val: request r's entries are
  * bias_indptr[r] .. bias_indptr[r+1] (NULL: none). allow
  * [n_allow][allow_words] bits (NULL: none): row t is under mask
  * allow_row[t], or under none if that is negative (a number that is not

@@ -811,6 +811,24 @@ def test_logits_not_numbers(cuda_lib):
         assert bool((y[0, 128:] == float("-inf")).all())
 
 
+def test_logits_too_many_drafts(cuda_lib):
+    """A request of more rows than drafts are followed for: reported, its rows
+    as without drafts, the other request's with them."""
+    wb, n = cuda_lib, 4097
+    draft = [t % 60 for t in range(n + 2)]
+    x = torch.ones(n + 2, 64)
+    y = torch.full_like(x, 7.0).cuda()
+    t = dict(logits=x.cuda(), q_indptr=dev([0, n, n + 2]), draft=dev(draft), freq=dev([0.5, 0.5], torch.float32))
+    wb.logits_adjust_dev(wb.LogitsAdjust(B=2, R=n + 2, V=64, dtype=wb.F32, tree_words=0, ld=64, ld_out=64, out=p(y),
+                                         **{k: p(v) for k, v in t.items()}), stream())
+    assert wb.device_errors() == wb.DERR_BAD_TREE
+    want = torch.ones(n + 2, 64)
+    for row in (n, n + 1):
+        for k in range(n, row + 1):
+            want[row, draft[k]] -= 0.5
+    assert torch.equal(y.cpu(), want)
+
+
 # ---- together ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

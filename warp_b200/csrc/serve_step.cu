@@ -328,6 +328,8 @@ constexpr int kLogHalf = kLogThreads / 2;
 constexpr int kLogSlice = 65536;     /* the widest slice                          */
 constexpr int kLogCap = 4096;
 constexpr int kLogDrafts = 256;      /* drafted tokens of a slice that are listed */
+constexpr int kLogBranch = 4096;     /* rows of a request that drafts are followed for:
+                                        without the list their cost grows with its square */
 constexpr int kLogRows = 4;          /* rows a CTA takes at most                  */
 constexpr int kLogKeep = 16;         /* tokens a thread keeps between its two uses */
 constexpr uint32_t kPrompt = 0x80000000u, kDrafted = 0x40000000u;
@@ -395,6 +397,8 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     const int hm = d.prompt_len ? d.prompt_len[r] : 0;
     const int *hist = d.hist + (size_t)r * d.hist_stride;
     const int b0 = d.bias_indptr ? max(d.bias_indptr[r], 0) : 0, bn = d.bias_indptr ? d.bias_indptr[r + 1] - b0 : 0;
+    const int nd = !d.draft || q1 - q0 > kLogBranch ? 0 : q1 - q0;
+    if (d.draft && q1 - q0 > kLogBranch && tid == 0 && blockIdx.x == 0) atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
     const int ht = tid - kLogHalf;                            /* of the half that counts     */
     /* what a thread needs twice is loaded once: under the copy a load takes long */
     int keep[kLogKeep], id_b = -1, id_d = -1;
@@ -408,7 +412,7 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
 #pragma unroll
         for (int k = 0; k < kLogKeep; k++) keep[k] = ht + k * kLogHalf < hn ? hist[ht + k * kLogHalf] : -1;
         if (ht < bn) id_b = d.bias_id[b0 + ht];
-        if (d.draft && ht < q1 - q0) id_d = d.draft[q0 + ht];
+        if (ht < nd) id_d = d.draft[q0 + ht];
         for (int i = ht; i < words; i += kLogHalf) s.named[i] = 0;
         if (ht == 0) s.nlist = 0;
     }
@@ -468,11 +472,10 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
             const int k = number(i == ht ? id_b : d.bias_id[b0 + i]);
             if (k >= 0) atomicMax(&s.bias[k], (uint32_t)(i + 1));
         }
-        if (d.draft)
-            for (int j = ht; j < q1 - q0; j += kLogHalf) {
-                const int k = number(j == ht ? id_d : d.draft[q0 + j]);
-                if (k >= 0) atomicOr(&s.cnt[k], kDrafted);
-            }
+        for (int j = ht; j < nd; j += kLogHalf) {
+            const int k = number(j == ht ? id_d : d.draft[q0 + j]);
+            if (k >= 0) atomicOr(&s.cnt[k], kDrafted);
+        }
     };
     if (ht < 0) {
         /* ---- the copy, row by row. Loaded words are not looked at before all loads
@@ -522,13 +525,12 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
         for (int i = ht + kLogKeep * kLogHalf; i < hn; i += kLogHalf) mark(hist[i]);
         mark(id_b);
         for (int i = ht + kLogHalf; i < bn; i += kLogHalf) mark(d.bias_id[b0 + i]);
-        if (d.draft)
-            for (int j = ht; j < q1 - q0; j += kLogHalf) {
-                const int id = j == ht ? id_d : d.draft[q0 + j];
-                if (!mark(id)) continue;
-                const int k = atomicAdd(&s.nlist, 1);
-                if (k < kLogDrafts) { s.list_j[k] = j; s.list_u[k] = id - v0; }
-            }
+        for (int j = ht; j < nd; j += kLogHalf) {
+            const int id = j == ht ? id_d : d.draft[q0 + j];
+            if (!mark(id)) continue;
+            const int k = atomicAdd(&s.nlist, 1);
+            if (k < kLogDrafts) { s.list_j[k] = j; s.list_u[k] = id - v0; }
+        }
         sync_half();
         if (numbered(0, words) <= kLogCap) counted(0, words);
     }
@@ -546,7 +548,7 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
             for (int k = 0; k < s.nlist; k++)
                 if (s.list_u[k] == u) n += on(t, s.list_j[k]);
         } else {
-            for (int j = 0; j < q1 - q0; j++)
+            for (int j = 0; j < nd; j++)
                 if (d.draft[q0 + j] == v0 + u) n += on(t, j);
         }
         return n;
