@@ -657,7 +657,8 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  * default stream. The calling thread's current device must be the one the
  * library is bound to. Lengths, ids and tables are read on the device
  * only; a value out of range there never moves an access outside the
- * caller's buffers: it raises a bit of waste_cuda_device_errors. A captured
+ * caller's buffers (but for bias_indptr below): it raises a bit of
+ * waste_cuda_device_errors. A captured
  * graph is valid until waste_cuda_shutdown.
  *
  * A new token t of request r is row t of the step's arrays, with
@@ -783,7 +784,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  * allow_row[t], or under none if that is negative (a number that is not
  * below n_allow raises BAD_MASK); allow_row NULL: mask t.
  * rep, freq, pres, hist NULL: 1, 0, 0, empty. Ids outside 0..V-1 are
- * ignored. ld, ld_out: elements between rows; out may be logits with the
+ * ignored; bias_indptr, whose lists have no length to hold it to, is
+ * believed as it is. ld, ld_out: elements between rows; out may be logits with the
  * same ld. Rows behind q_indptr[B] are left as they are. B up to 4096, R up
  * to 65535. */
 typedef struct {
