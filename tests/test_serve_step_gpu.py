@@ -775,6 +775,35 @@ def test_logits_many_named(cuda_lib, dtype):
         assert bool(((g - ref[t]).abs() <= tol)[fin].all())
 
 
+@pytest.mark.parametrize("n", [4095, 4097, 8191, 8192, 8193, 10000])
+@pytest.mark.parametrize("where", ["dense", "dense_end", "spread"])
+def test_logits_named_pieces(cuda_lib, n, where):
+    """As many named ids in a slice as are taken at once, one fewer and more:
+    side by side at either end, or all over it. Values and penalties are whole
+    numbers, so the results are exact."""
+    wb, V = cuda_lib, 40000
+    ids = {"dense": range(n), "dense_end": range(V - n, V), "spread": [i * 4 + i % 3 for i in range(n)]}[where]
+    hist = random.Random(n).sample(list(ids), n)
+    hist += hist[:50]
+    x = torch.arange(V, dtype=torch.float32).view(1, V).repeat(64, 1)
+    y = torch.full_like(x, 7.0).cuda()
+    # rows of one request, so that the slices are wide
+    t = dict(logits=x.cuda(), q_indptr=dev([0, 64]), hist=dev(hist), hist_len=dev([len(hist)]),
+             freq=dev([2.0], torch.float32), pres=dev([1.0], torch.float32))
+    for B in (1, 64):
+        if B == 64:                                              # and a row a request
+            t.update(q_indptr=dev(range(65)), hist=dev(hist * 64), hist_len=dev([len(hist)] * 64),
+                     freq=dev([2.0] * 64, torch.float32), pres=dev([1.0] * 64, torch.float32))
+        wb.logits_adjust_dev(wb.LogitsAdjust(B=B, R=64, V=V, dtype=wb.F32, hist_stride=len(hist), ld=V, ld_out=V, out=p(y),
+                                             **{k: p(v) for k, v in t.items()}), stream())
+        want = x[0].clone()
+        want[hist[:n]] -= 3
+        want[hist[:50]] -= 2
+        assert torch.equal(y.cpu(), want.expand(64, V)), B
+        y.fill_(7.0)
+    assert wb.device_errors() == 0
+
+
 def test_logits_mask_out_of_range(cuda_lib):
     wb = cuda_lib
     c = Logits(wb, 3, "f32", 500, [1, 1], 4, 2, use=("allow", "rows"), extra=0)

@@ -314,10 +314,14 @@ __global__ void __launch_bounds__(kRowsWarps * 32) mla_rows_kernel(
  * values again; a row's branch of drafted tokens is counted where a drafted id
  * is met. A count per named id and not per id lets the CTAs of a whole batch
  * be resident at once; where a slice's named ids are more than kLogCap they
- * are taken in pieces of kLogCap ids.
- * 64 rows of 163840 16-bit logits take 18 us (43 MB: 6.6 us of copying), 180
- * fp32 rows of 16 trees 78 us (247 MB: 38 us). Measured and slower: counts for
- * every id, in several waves (33 us), the rows staged in shared memory (67),
+ * are taken in the widest pieces that hold no more, each of which reads the
+ * history again. 4096 of them leave most of an SM's L1 to the history and the
+ * named values: with 8192, which two CTAs an SM still have room for, the cases
+ * below took 21 us, and 103 on either side of 4096 named ids.
+ * 64 rows of 163840 16-bit logits take 18 us (43 MB: 6.6 us of copying), 187
+ * fp32 rows of 16 trees 76 to 78 us (247 MB: 38 us) where no slice names more
+ * than kLogCap ids, and 102 to 105 where one does (165 with pieces of always
+ * kLogCap ids). Measured and slower: counts for every id, in several waves (33 us), the rows staged in shared memory (67),
  * the sparse half following the copy row by row (20 and 85), the sparse work
  * as a kernel of its own under the copy (24 and 94).
  *
@@ -592,15 +596,21 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
         for (int t = 0; t < rows; t++) again(t, total);
         return;
     }
-    for (int w0 = 0; w0 < words; w0 += kLogCap / 32) {
-        const int wn = min(kLogCap / 32, words - w0);
+    /* pieces as wide as fit: each reads the history again, so few of them. A piece
+     * of kLogCap ids always fits */
+    for (int w0 = 0, wn = (words + 1) / 2; w0 < words;) {
+        wn = min(wn, words - w0);
         __syncthreads();
-        if (ht >= 0) {
-            numbered(w0, wn);
-            counted(w0, wn);
+        if (ht >= 0 && numbered(w0, wn) <= kLogCap) counted(w0, wn);
+        __syncthreads();
+        const int n = s.n;
+        if (n > kLogCap) {
+            wn = (wn + 1) / 2;
+            continue;
         }
-        __syncthreads();
-        for (int t = 0; t < rows; t++) again(t, s.n);
+        for (int t = 0; t < rows; t++) again(t, n);
+        w0 += wn;
+        wn *= 2;
     }
 }
 
