@@ -486,7 +486,11 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  *   O^T [kl x N]        += C^T [kl x 128] . P^T          A M-major, same bytes
  * One copy of the tile in shared memory serves both. N is 32 where a
  * request's rows fit that, else 64: the cache is read once per 32 or 64 rows
- * (the second by 64: one token of 64 heads, or two of 32).
+ * (the second by 64: one token of 64 heads, or two of 32). The rule is the mean
+ * of the call's rows a request, which the host knows: 64 tokens of 32 heads in
+ * 64 requests take 61 us at N = 32 and 74 at 64; trees of up to 16 nodes 133
+ * and 109; 2 trees of up to 5 over 131003 rows 224 and 183; 512 tokens over
+ * 8192 rows 657 and 433.
  *
  * Shared memory (1 CTA an SM): a ring of 32 KB pairs (128 keys x 2 swizzled
  * 64-column chunks) that TMA fills page by page, 5 pairs at N = 32 and 4 at
@@ -505,15 +509,15 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  * memory over the 4 warps), the reference moved and O in TMEM rescaled.
  *
  * What bounds it. N = 32: 64 tokens over 183 k bf16 rows (216 MB) take 60 us
- * with the joining, 3.6 TB/s. Traced tiles took 6.7 to 7.5 k cycles, where
+ * with the joining (60 to 61 from run to run), 3.5 TB/s. Traced tiles took 6.7 to 7.5 k cycles, where
  * 147 KB at an SM's share of HBM would take 6.4 k. At some ten tiles a CTA that
  * accounts for 36 us or so; the start (lengths, table, first tile: loads that
  * wait for one another), the end and the joining are left with the rest. N =
  * 64, the chain of a tile in one SM's shared memory: a tile is loaded (from L2:
  * 2.5 k cycles at 64 rows a box, 3.4 k at 32), its scores (36 products of 48
  * cycles, under the loads), the softmax 1.5 k, the second product 1.6 k. 512
- * tokens of 32 heads over 8192 rows take 429 us, 702 TFLOP/s; trees of 16 nodes
- * for 16 requests 108 us. Measured and slower: V loaded again instead of held,
+ * tokens of 32 heads over 8192 rows take 433 us, 696 TFLOP/s; trees of up to 16
+ * nodes for 16 requests 109 us. Measured and slower: V loaded again instead of held,
  * for an N of 96 (554 us where N = 64 took 445), rows sent for towards L2 two
  * tiles ahead (64 tokens: 62 -> 70 us).
  *
@@ -1424,7 +1428,9 @@ extern "C" {
  * 64-column chunks, a rope part of at most one, and rows that 16-byte copies
  * can start at (0: the other kernel's). Where pages are whole 8-row swizzle
  * groups TMA loads them, in boxes of 64 columns by the returned number of
- * rows; 1: they are copied row by row. */
+ * rows; 1: they are copied row by row, which takes two to three times as long
+ * (64 tokens over up to 4096 rows each: 61 us by TMA, 140 by rows; 512 tokens
+ * over 8192 rows: 433 and 1330). */
 int wc_mla_tree_box(const waste_cuda_mla_tree_desc *d)
 {
     const uintptr_t addr = (uintptr_t)d->q | (uintptr_t)d->cache;
