@@ -644,6 +644,25 @@ def test_attn_decreasing_indptr(cuda_lib, name):
     assert bool((a.go == 7).all()) and bool((a.gl == 7).all())
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("name", ["chains", "unserved", "unserved_one"])
+def test_attn_segments_without_keys(cuda_lib, name, dtype):
+    """Several segments a CTA, some of them without keys (the units that a
+    chain's closed count adds; requests that were not served), so that what one
+    segment left under way meets the next one's queries."""
+    if name == "chains":
+        a = Attn(cuda_lib, 21, dtype, 16, 128, 32, 64, [309, 242, 320, 297, 33], [50, 95, 89, 36, 67])
+    else:
+        n = 300
+        a = Attn(cuda_lib, 22, dtype, 32, 128, 32, 16, [(37 * r) % 90 for r in range(n)], [2 if name == "unserved" else 1] * n,
+                 unserved=[r for r in range(n) if r % 3])
+    ref = a.ref()
+    a.put()
+    for _ in range(3):
+        a.go.fill_(7.0)
+        a.call().check(ref)
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

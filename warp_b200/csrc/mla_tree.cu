@@ -310,7 +310,9 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
             s.tok[tid] = (g.row0 + tid) / H;
         }
         __syncthreads();
-        {
+        /* a segment without keys waits for no copies, so it issues none: they would be
+         * under way when the next segment's go to the same place */
+        if (g.k0 < g.k1) {
             const int i = tid >> 3, tok = s.tok[i], h = g.row0 + i - tok * H;
             const T *src = static_cast<const T *>(d.q);
             if (i < rows) src += (size_t)(g.q.q0 + tok) * d.q_token_stride + (size_t)h * d.q_head_stride;
