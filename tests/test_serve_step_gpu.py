@@ -663,6 +663,43 @@ def test_attn_segments_without_keys(cuda_lib, name, dtype):
         a.call().check(ref)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("H", [32, 64])
+@pytest.mark.parametrize("unit", [23, 24, 25, 26, 27, 28])
+def test_attn_coarse_scores(cuda_lib, unit, H, dtype):
+    """Scores where 32 bits step by 1 to 32: the difference to the reference of
+    the tiles before, and that reference, are not exact there, and a weight may
+    not leave the type for it. Scores are exact: products of powers of two plus
+    whole steps, 128 keys a score, each next score larger by 8 in units of log2
+    (or the step). 160 requests of three tiles, so that a CTA has several in a row."""
+    step = max(8, 2 ** (unit - 23))
+    for first in range(1, 8):                        # steps from the power of two: odd and even last bits
+        a = Attn(cuda_lib, 3, dtype, H, 128, 64, 64, [383] * 160, [1] * 160, None)
+        a.table[:] = a.table[0]
+        a.scale = float(np.float32(np.log(2.0)))     # units of log2 (to 2^-24)
+        a.q[:] = 0
+        a.q[:, :, 0], a.q[:, :, 1] = 2.0 ** 13, 1.0
+        a.cache[:] = torch.randn(a.cache.shape, generator=torch.Generator().manual_seed(first)).to(a.cache.dtype)
+        rows = torch.from_numpy(a.table[0]).long()
+        flat = a.cache[rows].view(-1, a.D)
+        flat[:, 0] = 2.0 ** (unit - 13)
+        flat[:128, 1] = first * 2.0 ** max(0, unit - 23)
+        flat[128:256, 1] = first * 2.0 ** max(0, unit - 23) + step
+        flat[256:, 1] = first * 2.0 ** max(0, unit - 23) + 2 * step
+        a.cache[rows] = flat.view(len(rows), a.page, a.D)
+        a.put().call()
+        torch.cuda.synchronize()
+        # weights 2^-2step, 2^-step and 1, exact but for the scale's 2^-24 of 16
+        w = torch.exp2(-float(step) * torch.tensor([2.0, 1.0, 0.0], dtype=torch.float64)).repeat_interleave(128)
+        lat = flat[:, :128].double()
+        want = (w @ lat) / w.sum()
+        size = (w @ lat.abs()) / w.sum()
+        tol = size * (2 * HALF[dtype] + 1e-5) + 2.0 ** -30
+        got = a.go[:a.T].cpu().double()
+        assert bool(((got - want).abs() <= tol).all()), first
+    assert cuda_lib.device_errors() == 0
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

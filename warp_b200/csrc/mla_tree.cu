@@ -1095,9 +1095,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     bar_named(1 + quarter, 128);
                     mx = fmaxf(fmaxf(sx[0][lc], sx[1][lc]), fmaxf(sx[2][lc], sx[3][lc]));
                     float a = 1.0f;
-                    if (mx > r + (kBias + kLazy)) {
-                        a = ex2(r - (mx - kBias));
-                        r = mx - kBias;
+                    /* the same difference that the vote saw, and a reference not below
+                     * mx - kBias: from 2^25 on sums with these constants round, and a
+                     * weight of 2^16 is no fp16 */
+                    if (__fsub_rn(mx, r) > kBias + kLazy) {
+                        const float to = __fsub_ru(mx, kBias);
+                        a = ex2(r - to);
+                        r = to;
                     }
                     if (lane < NC) { mine[0][lane] = a; mine[1][lane] = r; }
                     bar_named(1 + quarter, 128);              /* and sx is read              */
