@@ -686,11 +686,14 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  *              its input's array
  *   block_table   the new entries are written, the others left as they are
  *   q_indptr [B+1], kv_len [B] (rows with the new ones), pos [T] (rotary
- *   position: ctx + depth; ctx for nodes past 32 * mask_words), slot [T] (cache row), mask [T][mask_words]
- *   (bit j: node j is an ancestor or the node itself; NULL allowed with a
- *   chain), short_blocks [1] (blocks that lacked, 0 if none).
+ *   position: ctx + depth; ctx for nodes past 32 * mask_words), slot [T]
+ *   (cache row), mask [T][mask_words] (bit j: node j is an ancestor or the
+ *   node itself; NULL allowed with a chain), short_blocks [1] (blocks that
+ *   lacked, 0 if none).
  * T: rows of the per-token arrays; rows behind the last request's are left
- * as they are. B <= 4096; q <= 32 * mask_words where a mask is written. */
+ * as they are. New tokens past T are left out (BAD_TREE): q_indptr and kv_len
+ * count those that have a row, the blocks are taken for all. B <= 4096;
+ * q <= 32 * mask_words where a mask is written. */
 typedef struct {
     int B, T, page, max_blocks, n_free, mask_words;
     const int *ctx_len, *q_len, *parent, *free_blocks, *free_head, *n_blocks;

@@ -700,6 +700,27 @@ def test_attn_coarse_scores(cuda_lib, unit, H, dtype):
     assert cuda_lib.device_errors() == 0
 
 
+def test_plan_cut_at_T(cuda_lib):
+    """More new tokens than rows, in the middle of a request: the request has
+    the rows that are there, its length counts those, and a chain planned so
+    sees its cached rows and itself, none of the rows that nobody wrote."""
+    wb = cuda_lib
+    ctx, q, page = [0, 5, 3], [3, 6, 2], 4
+    a = Attn(wb, 6, "bf16", 32, 512, 64, page, ctx, [3, 2, 0], None, extra=0)
+    pl = Plan(wb, ctx, q, [0, 2, 1], [[-1, -1, -1], [8, 9, -1], [7, -1, -1]], list(range(7)), 0, page, 1, None, extra=-6)
+    wb.kv_plan_dev(pl.d, stream())
+    assert wb.device_errors() == wb.DERR_BAD_TREE
+    assert pl.t["q_indptr"].tolist() == [0, 3, 5, 5]
+    assert pl.t["kv_len"].tolist() == [3, 7, 3]
+    assert pl.t["slot"].tolist() == [0, 1, 2, 9 * page + 1, 9 * page + 2]
+    a.table, a.kv = np.asarray(pl.t["block_table"].cpu(), np.int64), [3, 7, 3]
+    a.cache = torch.randn(10, page, a.D, generator=torch.Generator().manual_seed(1)).to(a.cache.dtype)
+    a.n_blocks = 10
+    a.put()
+    a.d.block_table, a.d.kv_len, a.d.q_indptr = (p(pl.t[k]) for k in ("block_table", "kv_len", "q_indptr"))
+    a.call().check()
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

@@ -133,8 +133,11 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(
             if (k >= per || r >= d.B) continue;
             const bool served = s.fstart[r] >= 0;
             d.n_blocks_out[r] = held[k] + (served ? need[k] : 0);
-            d.kv_len[r] = served ? d.ctx_len[r] + q[k] : 0;
-            d.q_indptr[r + 1] = min(s.qstart[r + 1], d.T);
+            /* the rows with the new ones that have one of T's: a longer length would
+             * make cached rows of those that are there */
+            const int end = min(s.qstart[r + 1], d.T);
+            d.kv_len[r] = served ? d.ctx_len[r] + (end - min(s.qstart[r], d.T)) : 0;
+            d.q_indptr[r + 1] = end;
         }
         if (tid == 0) {
             d.q_indptr[0] = 0;
