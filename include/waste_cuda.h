@@ -712,7 +712,10 @@ int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream);
  * rope values rotated in pairs (2j, 2j+1) by pos[t] * inv_freq[j]
  * (inv_freq NULL: NoPE), and kl + rope values are rounded to `dtype` into
  * cache row slot[t] (row_stride elements apart; n_rows rows). A negative
- * slot skips its token; slots of one call are distinct. Sums, angles and
+ * slot skips its token; slots of one call are distinct. n_tokens: rows of T
+ * that are there, read on the device (NULL: all T; kv_plan's q_indptr + B, in
+ * a step captured once and replayed with fewer tokens, whose rows behind keep
+ * an earlier step's slots; outside 0..T: BAD_BLOCK, nothing written). Sums, angles and
  * the rotation in at least 32 bits (the angle in 64). kl 1..4096, rope even,
  * 0..512. */
 typedef struct {
@@ -726,6 +729,7 @@ typedef struct {
     void *cache;
     size_t row_stride;
     int64_t n_rows;
+    const int *n_tokens;                         /* [1]                   */
 } waste_cuda_mla_rows_desc;
 int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
 

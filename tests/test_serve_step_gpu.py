@@ -1011,3 +1011,90 @@ def test_step_together(cuda_lib, dtype):
         held, table, head = ref["n_blocks"], ref["table"], ref["head"]
         ctx = [c + n for c, n in zip(ctx, q)] if step == 0 else ctx
     assert wb.device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_step_captured_with_fewer_tokens(cuda_lib, dtype):
+    """A whole step captured at T rows and replayed with fewer tokens, then with
+    T again: the rows behind the last token are no token's, whatever slots and
+    latents an earlier step left there, so kept rows stay what they were."""
+    wb = cuda_lib
+    rng, g = random.Random(8), torch.Generator().manual_seed(8)
+    B, H, kl, rope, page, cols, V, T = 3, 32, 512, 64, 4, 10, 300, 12
+    D, dt, pool = kl + rope, DT[dtype], 26
+    cache = torch.zeros(pool, page, D, dtype=dt, device="cuda")
+    free = list(range(pool))
+    rng.shuffle(free)
+    held, table, head, ctx = [0] * B, np.full((B, cols), -1), 0, [0] * B
+    pl = Plan(wb, ctx, [4] * B, held, table, free, head, page, 1, None, extra=0, inplace=True)
+    w = 1 + 0.1 * torch.randn(kl, generator=g)
+    inv = 10000.0 ** (-torch.arange(0, rope, 2).float() / rope)
+    gx, gw, gi = torch.zeros(T, D, device="cuda"), w.cuda(), inv.cuda()
+    gq = torch.zeros(T, H, D, dtype=dt, device="cuda")
+    o, lse = torch.empty(T, H, kl, dtype=dt, device="cuda"), torch.empty(T, H, device="cuda")
+    raw, out = torch.zeros(T, V, device="cuda"), torch.empty(T, V, device="cuda")
+    freq, draft = dev([0.5] * B, torch.float32), dev([0] * T)
+    n = wb.mla_tree_ws_bytes(H, kl)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    t = pl.t
+    calls = [
+        (wb.kv_plan_dev, pl.d),
+        (wb.mla_rows_dev, wb.MlaRows(
+            T=T, kl=kl, rope=rope, x_dtype=0, dtype=CODE[dtype], x_stride=D, x=p(gx), norm_w=p(gw), inv_freq=p(gi),
+            pos=p(t["pos"]), slot=p(t["slot"]), eps=1e-6, cache=p(cache), row_stride=D, n_rows=pool * page,
+            n_tokens=p(t["q_indptr"]) + 4 * B)),
+        (wb.mla_tree_attn_dev, wb.MlaTree(
+            B=B, T=T, heads=H, kl=kl, rope=rope, dtype=CODE[dtype], page=page, max_blocks=cols, mask_words=1, n_blocks=pool,
+            row_stride=D, q_token_stride=H * D, q_head_stride=D, o_token_stride=H * kl, o_head_stride=kl, q=p(gq),
+            cache=p(cache), block_table=p(t["block_table"]), kv_len=p(t["kv_len"]), q_indptr=p(t["q_indptr"]),
+            mask=p(t["mask"]), scale=0.07, o=p(o), lse=p(lse), ws=p(ws), ws_bytes=n)),
+        (wb.logits_adjust_dev, wb.LogitsAdjust(
+            B=B, R=T, V=V, dtype=0, tree_words=1, ld=V, ld_out=V, logits=p(raw), out=p(out), q_indptr=p(t["q_indptr"]),
+            freq=p(freq), draft=p(draft), tree=p(t["mask"])))]
+    graph, s = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=s):
+        for f, d in calls:
+            f(d, stream())
+    known = torch.zeros(pool * page, D, dtype=torch.float64)
+    for q in ([4, 4, 4], [1, 0, 2], [0, 3, 0], [4, 4, 4], [0, 0, 0], [1, 1, 1]):
+        n = sum(q)
+        x, qq = torch.randn(T, D, generator=g), torch.randn(T, H, D, generator=g).to(dt)
+        y, ids = torch.randn(T, V, generator=g), [rng.randrange(V) for _ in range(T)]
+        gx.copy_(x), gq.copy_(qq), raw.copy_(y), draft.copy_(dev(ids))
+        o.fill_(7.0), lse.fill_(7.0), out.fill_(7.0)
+        t["ctx_len"].copy_(dev(ctx)), t["q_len"].copy_(dev(q))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ref = O.plan(ctx, q, held, table, free, head, page, T, 1, None, cols)
+        vals = O.rows(x[:n], w, inv, torch.tensor(ref["pos"]), 1e-6)
+        if n:
+            known[ref["slot"]] = vals
+        got = cache.view(-1, D).cpu().double()
+        # a row's rotated pairs are bounded by the pair's size, no more than the row's largest twice
+        tol = known.abs() * (HALF[dtype] + (kl / 2 + 8) * E) + TINY[dtype]
+        tol[:, kl:] += 24 * E * known[:, kl:].abs().amax(1, keepdim=True)
+        assert bool(((got - known).abs() <= tol).all()), q
+        if n:
+            ro, rl, to, tl = O.attn(qq[:n], cache.cpu(), ref["table"], ref["kv_len"], ref["q_indptr"], ref["mask"], 0.07, kl, page, dtype)
+            assert bool(((o[:n].cpu().double() - ro).abs() <= to).all())
+            assert bool(((lse[:n].cpu().double() - rl).abs() <= tl).all())
+            adj = O.logits(y[:n].double(), ref["q_indptr"], None, None, None, None, [0.5] * B, None, ids, ref["mask"], None, None, None)
+            assert bool(((out[:n].cpu().double() - adj).abs() <= (adj.abs() + 8 * y[:n].abs() + 8) * E).all())
+        assert bool((o[n:] == 7).all()) and bool((lse[n:] == 7).all()) and bool((out[n:] == 7).all())
+        held, table, head = ref["n_blocks"], ref["table"], ref["head"]
+        ctx = [c + k for c, k in zip(ctx, q)]
+    assert wb.device_errors() == 0
+
+
+@pytest.mark.parametrize("there,bad", [(0, 0), (2, 0), (5, 0), (6, 1), (-1, 1)])
+def test_rows_counted_on_device(cuda_lib, there, bad):
+    """n_tokens rows are written, of T; outside 0..T it is reported, nothing written."""
+    wb = cuda_lib
+    x, w, c = torch.randn(5, 80).cuda(), torch.ones(64).cuda(), torch.zeros(6, 80).cuda()
+    slot, n = dev([4, 1, 0, 3, 5], torch.int64), dev([there])
+    wb.mla_rows_dev(wb.MlaRows(T=5, kl=64, rope=16, x_dtype=0, dtype=0, x_stride=80, x=p(x), norm_w=p(w), slot=p(slot),
+                               eps=1e-6, cache=p(c), row_stride=80, n_rows=6, n_tokens=p(n)), stream())
+    assert wb.device_errors() == (wb.DERR_BAD_BLOCK if bad else 0)
+    wrote = (c != 0).any(1).tolist()
+    assert [r for r in range(6) if wrote[r]] == sorted([4, 1, 0, 3, 5][:0 if bad else there])

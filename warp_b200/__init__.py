@@ -105,7 +105,7 @@ class MlaRows(C.Structure):
                 [("x_stride", C.c_size_t)] +
                 [(n, C.c_void_p) for n in ("x", "norm_w", "inv_freq", "pos", "slot")] +
                 [("eps", C.c_float), ("cache", C.c_void_p), ("row_stride", C.c_size_t),
-                 ("n_rows", C.c_int64)])
+                 ("n_rows", C.c_int64), ("n_tokens", C.c_void_p)])
 
 
 class MlaTree(C.Structure):

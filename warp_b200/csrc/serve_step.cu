@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kRowsWarps * 32) mla_rows_kernel(
     if (t >= d.T) return;
     const TX *x = static_cast<const TX *>(d.x) + (size_t)t * d.x_stride;
     const int64_t slot = d.slot[t];
+    const int there = d.n_tokens ? *d.n_tokens : d.T;
     const int pos = d.inv_freq ? d.pos[t] : 0;
     Pack<TX, VEC> v[K];
     Pack<float, VEC> w[K];
@@ -256,8 +257,9 @@ __global__ void __launch_bounds__(kRowsWarps * 32) mla_rows_kernel(
         const int i = lane * VEC + kStep * k;
         if (i < d.kl) w[k] = *reinterpret_cast<const Pack<float, VEC> *>(d.norm_w + i);
     }
-    if (slot < 0 || slot >= d.n_rows) {
-        if (slot >= 0 && lane == 0) atomicOr(err, WASTE_CUDA_DERR_BAD_BLOCK);
+    const bool short_of = there < 0 || there > d.T;
+    if (short_of || t >= there || slot < 0 || slot >= d.n_rows) {
+        if ((short_of || (t < there && slot >= 0)) && lane == 0) atomicOr(err, WASTE_CUDA_DERR_BAD_BLOCK);
         return;
     }
     TC *y = static_cast<TC *>(d.cache) + (size_t)slot * d.row_stride;
