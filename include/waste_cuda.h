@@ -396,9 +396,11 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
 #define WASTE_CUDA_DERR_PEER_WAIT  8u   /* expert parallel: a peer's token or partial-sum
                                            flag did not arrive (a rank that did not make
                                            the call); the layer's outputs are not valid */
-#define WASTE_CUDA_DERR_BAD_BLOCK 16u  /* a paged-cache call met a block id, a cache row or a
-                                           length outside the cache or its table; that request's
-                                           results are not valid, nothing outside was touched */
+#define WASTE_CUDA_DERR_BAD_BLOCK 16u  /* a serving-step call met a block id, a cache row or a
+                                           length outside the cache, its table or its list; that
+                                           request's results are not valid, nothing outside was
+                                           touched. Or a q_indptr that decreases or leaves the
+                                           rows: that call wrote nothing */
 #define WASTE_CUDA_DERR_BAD_TREE  32u  /* kv_plan: a parent that is no earlier node (taken as a
                                            root), a tree of more than 32 * mask_words nodes (not
                                            served), or more new tokens than T (left out);
@@ -772,8 +774,9 @@ size_t waste_cuda_mla_tree_ws_bytes(int heads, int kl);
 int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream);
 
 /* Rows of logits made ready for sampling. Request r has rows
- * q_indptr[r] <= t < q_indptr[r+1] (q_indptr NULL: row r, R = B). In this
- * order, for each id v of a row (x in 32 bits, rounded to `dtype` at the
+ * q_indptr[r] <= t < q_indptr[r+1] (q_indptr NULL: row r, R = B); q_indptr
+ * does not decrease and lies in 0..R (else BAD_BLOCK, and the call writes
+ * nothing). In this order, for each id v of a row (x in 32 bits, rounded to `dtype` at the
  * end):
  *   if v was seen      x = x > 0 ? x / rep[r] : x * rep[r]
  *   x -= freq[r] * n(v) + pres[r] * (n(v) > 0)    n: times v was produced
@@ -781,7 +784,7 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  *        last holds)
  *   x = -infinity      where the row's grammar mask has no bit v
  * Seen are the request's tokens hist[r][0 .. hist_len[r]); produced are
- * those from prompt_len[r] on. draft [R] (NULL: none): the row's node's
+ * those from prompt_len[r] on (prompt_len NULL: all). draft [R] (NULL: none): the row's node's
  * drafted token; the tokens of the node and its ancestors (bits of
  * tree[t], tree_words words; NULL: the rows up to its own) count as seen
  * and produced for that row (a request of more than 4096 rows: BAD_TREE, and

@@ -935,6 +935,18 @@ def test_logits_too_many_drafts(cuda_lib):
     assert torch.equal(y.cpu(), want)
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("ptr", [[0, 5, 2, 6], [3, 1, 1, 1], [0, 2, 4, 12], [-1, 2, 4, 5], [0, 2 ** 31 - 1, 3, 6], [0, 4, 5, -2 ** 31]])
+def test_logits_row_ranges(cuda_lib, ptr, inplace):
+    """Ranges of rows that go backwards or leave 0..R: reported, nothing written."""
+    wb = cuda_lib
+    c = Logits(wb, 5, "f32", 3001, [2, 2, 2], 20, 4, inplace=inplace)
+    c.t["q_indptr"].copy_(dev(ptr))
+    wb.logits_adjust_dev(c.d, stream())
+    assert wb.device_errors() == wb.DERR_BAD_BLOCK
+    assert torch.equal(c.gy.cpu(), c.x if inplace else torch.full_like(c.x, 7.0))
+
+
 # ---- together ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -376,7 +376,17 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
         auto begin = [&](int i) { return min(max(d.q_indptr[i], 0), d.R); };
         auto chunks = [&](int i) { return (max(begin(i + 1) - begin(i), 0) + kLogRows - 1) / kLogRows; };
         int sum = 0;
-        for (int i = first; i < last; i++) sum += chunks(i);
+        bool wrong = false;
+        for (int i = first; i < last; i++) {
+            wrong |= d.q_indptr[i] < 0 || d.q_indptr[i + 1] < d.q_indptr[i] || d.q_indptr[i + 1] > d.R;
+            sum += chunks(i);
+        }
+        /* ranges that go backwards overlap, or have more chunks than the grid: every
+         * CTA sees them, none writes */
+        if (__any_sync(0xffffffffu, wrong)) {
+            if (tid == 0 && (blockIdx.x | blockIdx.y) == 0) atomicOr(err, WASTE_CUDA_DERR_BAD_BLOCK);
+            return;
+        }
         int at = sum;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -407,7 +417,9 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     const int *hist = d.hist + (size_t)r * d.hist_stride;
     const int b0 = d.bias_indptr ? max(d.bias_indptr[r], 0) : 0, bn = d.bias_indptr ? d.bias_indptr[r + 1] - b0 : 0;
     const int nd = !d.draft || q1 - q0 > kLogBranch ? 0 : q1 - q0;
-    if (d.draft && q1 - q0 > kLogBranch && tid == 0 && blockIdx.x == 0) atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
+    if (tid == 0 && blockIdx.x == 0) {
+        if (d.draft && q1 - q0 > kLogBranch) atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
+    }
     const int ht = tid - kLogHalf;                            /* of the half that counts     */
     /* what a thread needs twice is loaded once: under the copy a load takes long */
     int keep[kLogKeep], id_b = -1, id_d = -1;
