@@ -784,7 +784,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
  *        last holds)
  *   x = -infinity      where the row's grammar mask has no bit v
  * Seen are the request's tokens hist[r][0 .. hist_len[r]); produced are
- * those from prompt_len[r] on (prompt_len NULL: all). draft [R] (NULL: none): the row's node's
+ * those from prompt_len[r] on (prompt_len NULL: all). A hist_len outside
+ * 0..hist_stride is held to it (BAD_BLOCK). draft [R] (NULL: none): the row's node's
  * drafted token; the tokens of the node and its ancestors (bits of
  * tree[t], tree_words words; NULL: the rows up to its own) count as seen
  * and produced for that row (a request of more than 4096 rows: BAD_TREE, and

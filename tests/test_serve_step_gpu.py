@@ -947,6 +947,19 @@ def test_logits_row_ranges(cuda_lib, ptr, inplace):
     assert torch.equal(c.gy.cpu(), c.x if inplace else torch.full_like(c.x, 7.0))
 
 
+@pytest.mark.parametrize("n", [-1, 21])
+def test_logits_history_length(cuda_lib, n):
+    """A history's length outside its row is reported and held to it."""
+    wb = cuda_lib
+    c = Logits(wb, 6, "f32", 300, [1, 2], 20, 4)
+    c.hist_len[1] = max(0, min(20, n))
+    c.prompt_len[1] = 3
+    c.t["hist_len"][1], c.t["prompt_len"][1] = n, 3
+    wb.logits_adjust_dev(c.d, stream())
+    c.check()
+    assert wb.device_errors() == wb.DERR_BAD_BLOCK
+
+
 # ---- together ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -419,6 +419,7 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     const int nd = !d.draft || q1 - q0 > kLogBranch ? 0 : q1 - q0;
     if (tid == 0 && blockIdx.x == 0) {
         if (d.draft && q1 - q0 > kLogBranch) atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
+        if (d.hist && hn != d.hist_len[r]) atomicOr(err, WASTE_CUDA_DERR_BAD_BLOCK);
     }
     const int ht = tid - kLogHalf;                            /* of the half that counts     */
     /* what a thread needs twice is loaded once: under the copy a load takes long */
