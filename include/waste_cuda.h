@@ -404,7 +404,8 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
 #define WASTE_CUDA_DERR_BAD_TREE  32u  /* kv_plan: a parent that is no earlier node (taken as a
                                            root), a tree of more than 32 * mask_words nodes (not
                                            served), or more new tokens than T (left out);
-                                           logits_adjust: more than 4096 rows with drafts */
+                                           logits_adjust: more than 4096 rows with drafts, or more
+                                           than 32 * tree_words */
 #define WASTE_CUDA_DERR_BAD_MASK  64u  /* logits_adjust: a row's mask number is not below
                                            n_allow; the row was left without a mask */
 unsigned waste_cuda_device_errors(void);

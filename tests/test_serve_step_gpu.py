@@ -960,6 +960,20 @@ def test_logits_history_length(cuda_lib, n):
     assert wb.device_errors() == wb.DERR_BAD_BLOCK
 
 
+def test_logits_tree_too_narrow(cuda_lib):
+    """More nodes than the tree's words have bits: reported, the rest of the
+    nodes on no branch."""
+    wb = cuda_lib
+    c = Logits(wb, 7, "f32", 300, [40, 3], 20, 4)
+    c.tree = np.ascontiguousarray(c.tree[:, :1])
+    c.t["tree"] = u32(c.tree)
+    c.d.tree, c.d.tree_words = p(c.t["tree"]), 1
+    c.tree = np.concatenate([c.tree, np.zeros_like(c.tree)], 1)
+    wb.logits_adjust_dev(c.d, stream())
+    c.check()
+    assert wb.device_errors() == wb.DERR_BAD_TREE
+
+
 # ---- together ------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])

@@ -418,7 +418,8 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     const int b0 = d.bias_indptr ? max(d.bias_indptr[r], 0) : 0, bn = d.bias_indptr ? d.bias_indptr[r + 1] - b0 : 0;
     const int nd = !d.draft || q1 - q0 > kLogBranch ? 0 : q1 - q0;
     if (tid == 0 && blockIdx.x == 0) {
-        if (d.draft && q1 - q0 > kLogBranch) atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
+        if ((d.draft && q1 - q0 > kLogBranch) || (d.tree && q1 - q0 > 32 * d.tree_words))
+            atomicOr(err, WASTE_CUDA_DERR_BAD_TREE);
         if (d.hist && hn != d.hist_len[r]) atomicOr(err, WASTE_CUDA_DERR_BAD_BLOCK);
     }
     const int ht = tid - kLogHalf;                            /* of the half that counts     */
