@@ -752,7 +752,8 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * [T][heads][kl] and q [T][heads][kl + rope] at the given strides in
  * elements; rows behind q_indptr[B] are left as they are. kl 1..512, rope
  * 0..128, page >= 1, mask_words * 32 >= the most new tokens of a request.
- * q_indptr does not decrease (else BAD_BLOCK, and the call writes nothing).
+ * q_indptr does not decrease and lies in 0..T (else BAD_BLOCK, and the call
+ * writes nothing).
  * n_blocks: blocks in the cache. o overlaps no input. ws: waste_cuda_mla_tree_ws_bytes(heads,
  * kl) bytes on the device, 256-byte aligned, not shared by calls that may
  * overlap (another stream, another captured graph); nothing in it has to

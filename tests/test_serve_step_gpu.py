@@ -721,6 +721,19 @@ def test_plan_cut_at_T(cuda_lib):
     a.call().check()
 
 
+@pytest.mark.parametrize("name", ["tree", "f32_tree", "pages_5", "ragged"])
+def test_attn_token_ranges(cuda_lib, name):
+    """Token ranges outside 0..T: reported, nothing written."""
+    wb = cuda_lib
+    a = attn_case(wb, name).put()
+    for r, x in ((0, -1), (0, -2 ** 31), (-1, a.T + a.extra + 1), (-1, 2 ** 31 - 1), (1, 2 ** 31 - 1)):
+        a.gi.copy_(dev(a.indptr))
+        a.gi[r] = x
+        a.call()
+        assert wb.device_errors() == wb.DERR_BAD_BLOCK
+        assert bool((a.go == 7).all()) and bool((a.gl == 7).all())
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

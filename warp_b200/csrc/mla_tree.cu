@@ -130,10 +130,11 @@ template <int kWarps> __device__ __forceinline__ void walk_begin(const Shape &p,
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (p.d.B + kWarps * 32 - 1) / (kWarps * 32), r0 = tid * per;
     int sum = 0;
-    bool back = false;
+    bool wrong = false;
     for (int k = 0; k < per && r0 + k < p.d.B; k++) {
         const Req q = req_at(p, r0 + k);
-        back |= p.d.q_indptr[r0 + k + 1] < p.d.q_indptr[r0 + k];
+        const int a = p.d.q_indptr[r0 + k], b = p.d.q_indptr[r0 + k + 1];
+        wrong |= a < 0 || b < a || b > p.d.T;
         if (blockIdx.x == 0 && p.d.kv_len[r0 + k] > p.d.max_blocks * p.d.page)
             atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
         sum += unit_prefix(p, q, q.nt);
@@ -146,12 +147,13 @@ template <int kWarps> __device__ __forceinline__ void walk_begin(const Shape &p,
     }
     if (lane == 31) s.sum[warp] = at;
     /* requests whose tokens go backwards overlap, and their units could pass 32
-     * bits: every CTA sees them, none has work */
-    back = __syncthreads_or(back);
-    if (back && blockIdx.x == 0 && tid == 0) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+     * bits; tokens cut off at T would take others for cached ones: every CTA sees
+     * them, none has work */
+    wrong = __syncthreads_or(wrong);
+    if (wrong && blockIdx.x == 0 && tid == 0) atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
     int v = lane < kWarps ? s.sum[lane] : 0;
     int all = __reduce_add_sync(0xffffffffu, v);
-    if (back) all = 0;
+    if (wrong) all = 0;
     v = __reduce_add_sync(0xffffffffu, lane < warp ? v : 0);
     at += v - sum;
     const int G = min((int)gridDim.x, all), c = blockIdx.x;
