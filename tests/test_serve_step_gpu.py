@@ -734,6 +734,20 @@ def test_attn_token_ranges(cuda_lib, name):
         assert bool((a.go == 7).all()) and bool((a.gl == 7).all())
 
 
+@pytest.mark.parametrize("name", ["tree", "f32_tree"])
+def test_attn_negative_length(cuda_lib, name):
+    """A length below zero: reported, its tokens see nothing, the others' results stand."""
+    wb = cuda_lib
+    a = attn_case(wb, name)
+    a.kv[0] = 0
+    a.put()
+    a.gk[0] = -5
+    ref = a.ref()
+    a.call()
+    assert wb.device_errors() == wb.DERR_BAD_BLOCK
+    a.check(ref)
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

@@ -135,7 +135,8 @@ template <int kWarps> __device__ __forceinline__ void walk_begin(const Shape &p,
         const Req q = req_at(p, r0 + k);
         const int a = p.d.q_indptr[r0 + k], b = p.d.q_indptr[r0 + k + 1];
         wrong |= a < 0 || b < a || b > p.d.T;
-        if (blockIdx.x == 0 && p.d.kv_len[r0 + k] > p.d.max_blocks * p.d.page)
+        const int kv = p.d.kv_len[r0 + k];
+        if (blockIdx.x == 0 && (kv < 0 || kv > p.d.max_blocks * p.d.page))
             atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
         sum += unit_prefix(p, q, q.nt);
     }
