@@ -405,7 +405,8 @@ int  waste_cuda_ep_moe_block_rep_dev(int layer, int T, const float *d_h,
                                            root), a tree of more than 32 * mask_words nodes (not
                                            served), or more new tokens than T (left out);
                                            logits_adjust: more than 4096 rows with drafts, or more
-                                           than 32 * tree_words */
+                                           than 32 * tree_words; mla_tree_attn: more new tokens
+                                           than 32 * mask_words */
 #define WASTE_CUDA_DERR_BAD_MASK  64u  /* logits_adjust: a row's mask number is not below
                                            n_allow; the row was left without a mask */
 unsigned waste_cuda_device_errors(void);
@@ -751,7 +752,8 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * product with the rows (their sum and lse are of the unrounded ones). o is
  * [T][heads][kl] and q [T][heads][kl + rope] at the given strides in
  * elements; rows behind q_indptr[B] are left as they are. kl 1..512, rope
- * 0..128, page >= 1, mask_words * 32 >= the most new tokens of a request.
+ * 0..128, page >= 1, mask_words * 32 >= the most new tokens of a request
+ * (else BAD_TREE: the request's new rows past that are seen by none).
  * q_indptr does not decrease and lies in 0..T (else BAD_BLOCK, and the call
  * writes nothing).
  * n_blocks: blocks in the cache. o overlaps no input. ws: waste_cuda_mla_tree_ws_bytes(heads,

@@ -748,6 +748,24 @@ def test_attn_negative_length(cuda_lib, name):
     a.check(ref)
 
 
+@pytest.mark.parametrize("name", ["tree_wide", "f32_tree"])
+def test_attn_mask_too_narrow(cuda_lib, name):
+    """More new tokens than the mask's words have bits: reported, and the rows
+    without a bit are seen by none."""
+    wb = cuda_lib
+    dtype, H, (kl, rope), page, ctx, q, tree = ATTN[name]
+    a = Attn(wb, 3, dtype, H, kl, rope, page, [90, 5], [41, 3], 1)
+    a.mask = np.ascontiguousarray(a.mask[:, :1])
+    a.words = 1
+    a.put()
+    a.mask = np.concatenate([a.mask, np.zeros_like(a.mask)], 1)
+    a.call()
+    ref = a.ref()
+    torch.cuda.synchronize()
+    assert wb.device_errors() == wb.DERR_BAD_TREE
+    a.check(ref)
+
+
 # ---- logits --------------------------------------------------------------------------
 
 class Logits:

@@ -138,6 +138,7 @@ template <int kWarps> __device__ __forceinline__ void walk_begin(const Shape &p,
         const int kv = p.d.kv_len[r0 + k];
         if (blockIdx.x == 0 && (kv < 0 || kv > p.d.max_blocks * p.d.page))
             atomicOr(p.err, WASTE_CUDA_DERR_BAD_BLOCK);
+        if (blockIdx.x == 0 && p.d.mask && q.n > 32 * p.d.mask_words) atomicOr(p.err, WASTE_CUDA_DERR_BAD_TREE);
         sum += unit_prefix(p, q, q.nt);
     }
     int at = sum;
