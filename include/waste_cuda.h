@@ -745,8 +745,9 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * of mask[t] is set; with mask NULL, the rows up to the token's own
  * (a chain). A token that sees nothing (as in a request with kv_len <
  * q_len, e.g. one that kv_plan did not serve) gets o = 0 and lse =
- * -infinity. A kv_len below 0 or past the table is reported (BAD_BLOCK). What a row holds (a NaN, an infinity) reaches the tokens that
- * see it and no others.
+ * -infinity. A kv_len below 0 or past the table is reported (BAD_BLOCK).
+ * What a row holds (a NaN, an infinity) reaches the tokens that see it and no
+ * others.
  * q and o are of the cache's type `dtype`; scores, the softmax and sums in
  * 32 bits; with 16-bit types the weights are rounded to the type for the
  * product with the rows (their sum and lse are of the unrounded ones). o is

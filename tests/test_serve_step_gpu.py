@@ -1182,3 +1182,26 @@ def test_rows_counted_on_device(cuda_lib, there, bad):
     assert wb.device_errors() == (wb.DERR_BAD_BLOCK if bad else 0)
     wrote = (c != 0).any(1).tolist()
     assert [r for r in range(6) if wrote[r]] == sorted([4, 1, 0, 3, 5][:0 if bad else there])
+
+
+def test_errors_raised_while_read(cuda_lib):
+    """A bit raised on one stream while another kind is read and cleared is still
+    there afterwards: every step's two faults are reported, by then at the latest."""
+    wb = cuda_lib
+    x, w, c, slot = torch.randn(1, 80).cuda(), torch.ones(64).cuda(), torch.zeros(1, 80).cuda(), dev([1], torch.int64)
+    rows = wb.MlaRows(T=1, kl=64, rope=16, x_dtype=0, dtype=0, x_stride=80, x=p(x), norm_w=p(w), slot=p(slot), eps=1e-6,
+                      cache=p(c), row_stride=80, n_rows=1)
+    y, a, row = torch.randn(1, 32).cuda(), u32([[1]]), dev([1])
+    adj = wb.LogitsAdjust(B=1, R=1, V=32, dtype=0, allow_words=1, n_allow=1, ld=32, ld_out=32, logits=p(y), out=p(y),
+                          allow=p(a), allow_row=p(row))
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for k in range(300):
+        wb.mla_rows_dev(rows, s1.cuda_stream)
+        s1.synchronize()
+        wb.logits_adjust_dev(adj, s2.cuda_stream)
+        got = wb.device_errors()
+        s2.synchronize()
+        got |= wb.device_errors()
+        assert got == wb.DERR_BAD_BLOCK | wb.DERR_BAD_MASK, k
+    assert wb.device_errors() == 0

@@ -633,6 +633,8 @@ __global__ void __launch_bounds__(kLogThreads, 2) logits_kernel(const waste_cuda
     }
 }
 
+__global__ void clear_bits_kernel(unsigned int *word, unsigned int bits) { atomicAnd(word, ~bits); }
+
 template <typename TX, typename TC>
 cudaError_t rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, cudaStream_t s)
 {
@@ -726,6 +728,13 @@ int wc_logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, int sms
     if (d->dtype == WASTE_CUDA_F32) return (int)logits_launch<float>(d, err, sms, s);
     if (d->dtype == WASTE_CUDA_F16) return (int)logits_launch<__half>(d, err, sms, s);
     return (int)logits_launch<__nv_bfloat16>(d, err, sms, s);
+}
+
+int wc_clear_bits_launch(unsigned int *word, unsigned int bits, void *stream)
+{
+    clear_bits_kernel<<<1, 1, 0, (cudaStream_t)stream>>>(word, bits);
+    wc_count_launches(1);
+    return (int)cudaGetLastError();
 }
 
 } /* extern "C" */

@@ -267,9 +267,14 @@ unsigned waste_cuda_device_errors(void)
     pthread_mutex_lock(&g_mu);
     unsigned v = S.inited ? read_device_errors(1) : 0;
     if (S.inited && v != ~0u) {
+        /* calls on other streams may raise bits meanwhile: only those reported are
+         * cleared */
         unsigned int w = 0;
-        if (cudaMemcpy(&w, S.d_serr, sizeof w, cudaMemcpyDeviceToHost) != cudaSuccess) v = ~0u;
-        else if (w) { memset_now(S.d_serr, 0, sizeof w); v |= w; }
+        if (cudaMemcpy(&w, S.d_serr, sizeof w, cudaMemcpyDeviceToHost) != cudaSuccess ||
+            (w && (wc_clear_bits_launch(S.d_serr, w, NULL) != 0 || cudaStreamSynchronize(0) != cudaSuccess)))
+            v = ~0u;
+        else
+            v |= w;
     }
     pthread_mutex_unlock(&g_mu);
     return v;

@@ -372,6 +372,8 @@ int    wc_mla_tree_launch(const waste_cuda_mla_tree_desc *d, const CUtensorMap *
                           unsigned int *err, int sms, void *stream);
 int    wc_logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, int sms,
                         void *stream);
+/* *word &= ~bits, atomically. */
+int    wc_clear_bits_launch(unsigned int *word, unsigned int bits, void *stream);
 
 /* Phase timers (see waste_cuda_profile in include/waste_cuda.h). */
 enum { WC_PH_ROUTER, WC_PH_ACT, WC_PH_GATEUP, WC_PH_DOWN, WC_PH_COMBINE,
