@@ -687,8 +687,12 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  *              its request's new tokens, smaller than its own, or -1 for a
  *              child of the last cached token.
  *   n_blocks_out, free_head_out   the counts after the step; each may be
- *              its input's array
- *   block_table   the new entries are written, the others left as they are
+ *              its input's array; no other output may share an element with
+ *              an input or another output
+]
+
+
+@pytest.mark.parametrize("name,make,wrong", REFUSED, *   block_table   the new entries are written, the others left as they are
  *   q_indptr [B+1], kv_len [B] (rows with the new ones), pos [T] (rotary
  *   position: ctx + depth; ctx for nodes past 32 * mask_words), slot [T]
  *   (cache row), mask [T][mask_words] (bit j: node j is an ancestor or the

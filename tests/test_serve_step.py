@@ -77,6 +77,10 @@ REFUSED = [
     ("logits_adjust_dev", logits, dict(tree_words=0)), ("logits_adjust_dev", logits, dict(bias_val=None)),
     ("logits_adjust_dev", logits, dict(allow_words=31)), ("logits_adjust_dev", logits, dict(logits=A, out=A, ld_out=1004)),
     ("logits_adjust_dev", logits, dict(out=A + 2)),
+    ("kv_plan_dev", plan, dict(pos=A, ctx_len=A)), ("kv_plan_dev", plan, dict(slot=A + 8, q_len=A + 36)),
+    ("kv_plan_dev", plan, dict(mask=A, parent=A + 12)), ("kv_plan_dev", plan, dict(block_table=A, free_blocks=A + 60)),
+    ("kv_plan_dev", plan, dict(short_blocks=A, free_head=A)), ("kv_plan_dev", plan, dict(free_head_out=A + 4, n_blocks=A)),
+    ("kv_plan_dev", plan, dict(pos=A, slot=A)), ("kv_plan_dev", plan, dict(n_blocks_out=A, kv_len=A)),
 ]
 
 
@@ -91,6 +95,17 @@ def test_refused(lib, name, make, wrong):
 def test_null_descriptors(lib):
     for n in ("kv_plan_dev", "mla_rows_dev", "mla_tree_attn_dev", "logits_adjust_dev"):
         assert getattr(lib, "waste_cuda_" + n)(None, None) == wb.E_ARG
+
+
+def test_plan_counts_in_place(lib):
+    """What the counts may share passes the checks (and asks for a device)."""
+    if wb.load_library().waste_cuda_device() >= 0:
+        pytest.skip("another test bound the library")
+    for kw in (dict(n_blocks=A, n_blocks_out=A), dict(free_head=A, free_head_out=A), dict(T=0, pos=A, ctx_len=A),
+               dict(n_free=0, free_blocks=A, kv_len=A)):
+        with pytest.raises(wb.WasteCudaError) as e:
+            wb.kv_plan_dev(plan(**kw))
+        assert e.value.rc == wb.E_NODEV, kw
 
 
 def test_nothing_to_do(lib):

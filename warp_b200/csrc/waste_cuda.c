@@ -3312,10 +3312,10 @@ static size_t dtype_size(int dtype)
 
 static int misaligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 
-/* n bytes at a and m at b share some */
+/* n bytes at a and m at b share some (an empty one with none) */
 static int overlap(const void *a, size_t n, const void *b, size_t m)
 {
-    return (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
+    return n && m && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
 }
 
 /* The caller holds g_mu: the library is bound and its device is current. */
@@ -3340,15 +3340,25 @@ int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream)
         return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: bad sizes or a missing array (B 1..4096)");
     if ((d->mask && d->mask_words < 1) || (d->parent && !d->mask))
         return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: a tree needs a mask of mask_words >= 1");
-    const size_t nb = (size_t)d->B * sizeof(int);
-    int *const outs[3] = { d->kv_len, d->q_indptr, d->n_blocks_out };
-    for (int k = 0; k < 3; k++) {
-        const size_t n = k == 1 ? nb + sizeof(int) : nb;
-        if (overlap(outs[k], n, d->ctx_len, nb) || overlap(outs[k], n, d->q_len, nb) ||
-            (overlap(outs[k], n, d->n_blocks, nb) && outs[k] != d->n_blocks) ||
-            (k < 2 && outs[k] == d->n_blocks))
-            return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: only the counts may be updated in place");
-    }
+    /* the arrays, outputs first: none shares an element with another but a count
+     * with the one that it updates */
+    const size_t nb = (size_t)d->B * sizeof(int), nt = (size_t)d->T * sizeof(int);
+    const struct { const void *p; size_t n; } a[] = {
+        { d->n_blocks_out, nb }, { d->free_head_out, sizeof(int) }, { d->block_table, nb * (size_t)d->max_blocks },
+        { d->q_indptr, nb + sizeof(int) }, { d->kv_len, nb }, { d->pos, nt }, { d->slot, 2 * nt },
+        { d->mask, nt * (size_t)(d->mask ? d->mask_words : 0) }, { d->short_blocks, sizeof(int) },
+        { d->ctx_len, nb }, { d->q_len, nb }, { d->parent, nt },
+        { d->free_blocks, (size_t)d->n_free * sizeof(int) }, { d->free_head, sizeof(int) }, { d->n_blocks, nb },
+    };
+    enum { kOuts = 9, kArrays = sizeof a / sizeof *a };
+    for (int i = 0; i < kOuts; i++)
+        for (int j = i + 1; j < kArrays; j++) {
+            if (a[i].p == a[j].p && ((a[i].p == d->n_blocks_out && j == kArrays - 1) ||
+                                     (a[i].p == d->free_head_out && j == kArrays - 2)))
+                continue;
+            if (a[i].p && a[j].p && overlap(a[i].p, a[i].n, a[j].p, a[j].n))
+                return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: only the counts may be updated in place");
+        }
     if (misaligned(d->slot, 8)) return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: slot is not 8-byte aligned");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("kv_plan_dev"))) goto out;
