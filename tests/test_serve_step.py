@@ -81,6 +81,8 @@ REFUSED = [
     ("kv_plan_dev", plan, dict(mask=A, parent=A + 12)), ("kv_plan_dev", plan, dict(block_table=A, free_blocks=A + 60)),
     ("kv_plan_dev", plan, dict(short_blocks=A, free_head=A)), ("kv_plan_dev", plan, dict(free_head_out=A + 4, n_blocks=A)),
     ("kv_plan_dev", plan, dict(pos=A, slot=A)), ("kv_plan_dev", plan, dict(n_blocks_out=A, kv_len=A)),
+    ("kv_plan_dev", plan, dict(mask_words=1 << 26)), ("mla_tree_attn_dev", tree, dict(mask_words=1 << 26)),
+    ("logits_adjust_dev", logits, dict(tree_words=1 << 26)),
 ]
 
 

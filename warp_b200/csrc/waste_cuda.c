@@ -3312,6 +3312,9 @@ static size_t dtype_size(int dtype)
 
 static int misaligned(const void *p, size_t n) { return ((uintptr_t)p & (n - 1)) != 0; }
 
+/* words of a row of bits, which the kernels number in 32 bits */
+static int words_ok(int words) { return words >= 1 && words <= INT32_MAX / 32; }
+
 /* n bytes at a and m at b share some (an empty one with none) */
 static int overlap(const void *a, size_t n, const void *b, size_t m)
 {
@@ -3338,8 +3341,8 @@ int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream)
         !d->n_blocks || !d->block_table || !d->free_head_out || !d->n_blocks_out || !d->q_indptr ||
         !d->kv_len || (d->T > 0 && (!d->pos || !d->slot)) || !d->short_blocks)
         return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: bad sizes or a missing array (B 1..4096)");
-    if ((d->mask && d->mask_words < 1) || (d->parent && !d->mask))
-        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: a tree needs a mask of mask_words >= 1");
+    if ((d->mask && !words_ok(d->mask_words)) || (d->parent && !d->mask))
+        return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: a tree needs a mask of mask_words 1..2^26 - 1");
     /* the arrays, outputs first: none shares an element with another but a count
      * with the one that it updates */
     const size_t nb = (size_t)d->B * sizeof(int), nt = (size_t)d->T * sizeof(int);
@@ -3411,7 +3414,7 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
     if (d->B == 0 || d->T == 0) return 0;
     const size_t z = dtype_size(d->dtype);
     if (!d->q || !d->cache || !d->block_table || !d->kv_len || !d->q_indptr || !d->o || !d->ws ||
-        (d->mask && d->mask_words < 1) || misaligned(d->q, z) || misaligned(d->cache, z) ||
+        (d->mask && !words_ok(d->mask_words)) || misaligned(d->q, z) || misaligned(d->cache, z) ||
         misaligned(d->o, z) || misaligned(d->ws, 256) || d->o == d->q || d->o == d->cache)
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
     pthread_mutex_lock(&g_mu);
@@ -3464,7 +3467,7 @@ int waste_cuda_logits_adjust_dev(const waste_cuda_logits_desc *d, void *stream)
         return fail(WASTE_CUDA_E_ARG, "logits_adjust_dev: bad sizes, type or strides (B up to 4096, R up to 65535)");
     if (d->B == 0 || d->R == 0) return 0;
     if (!d->logits || !d->out || (d->out == d->logits && d->ld != d->ld_out) ||
-        (d->hist && !d->hist_len) || (d->tree && (!d->draft || d->tree_words < 1)) ||
+        (d->hist && !d->hist_len) || (d->tree && (!d->draft || !words_ok(d->tree_words))) ||
         (d->bias_indptr && (!d->bias_id || !d->bias_val)) ||
         (d->allow && ((int64_t)d->allow_words * 32 < d->V || d->n_allow < 0)) ||
         misaligned(d->logits, dtype_size(d->dtype)) || misaligned(d->out, dtype_size(d->dtype)))
