@@ -681,7 +681,8 @@ int    waste_cuda_vq_matvec_sel_dev(int G, const uint8_t *const *idx,
  * free_blocks[*free_head ..), requests in ascending order. A request whose
  * share does not fit what is left, behind all before it, is not served
  * (and takes nothing): kv_len 0, slots -1. Neither is one whose blocks
- * exceed max_blocks or whose lengths are negative (BAD_BLOCK).
+ * exceed max_blocks or whose lengths are negative (BAD_BLOCK). A *free_head
+ * below 0 is taken as 0, one above n_free leaves no block (both BAD_BLOCK).
  *   parent     NULL: the new tokens are a chain (a prompt's chunk, or one
  *              token). Else [T]: the parent of each node as an index among
  *              its request's new tokens, smaller than its own, or -1 for a

@@ -189,6 +189,21 @@ def test_plan_tree_too_large(cuda_lib):
     assert pl.t["pos"].tolist() == [5 + i for i in range(32)] + [5] * 68
 
 
+@pytest.mark.parametrize("head,taken", [(-1, [4]), (5, [-1]), (2 ** 31 - 1, [-1]), (-2 ** 31, [4])])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_plan_free_head_outside(cuda_lib, head, taken, inplace):
+    """A head outside the free list is reported; requests that hold their
+    blocks are served all the same."""
+    wb = cuda_lib
+    pl = Plan(wb, [3, 2, 1], [1, 3, 1], [1, 1, 1], [[9, -1], [8, -1], [3, -1]], [4, 5, 6, 7], head, 4, 1, None, extra=0, inplace=inplace)
+    wb.kv_plan_dev(pl.d, stream())
+    assert wb.device_errors() == wb.DERR_BAD_BLOCK
+    assert pl.t["kv_len"].tolist() == [4, 5 if taken[0] >= 0 else 0, 2]
+    assert pl.t["block_table"].tolist() == [[9, -1], [8] + taken, [3, -1]]
+    assert pl.t["free_head_out"].tolist() == [1 if head < 0 else head]
+    assert pl.t["short_blocks"].tolist() == [0 if head < 0 else 1]
+
+
 # ---- rows ----------------------------------------------------------------------------
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])

@@ -65,7 +65,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(
     int q[kPlanPer], need[kPlanPer], held[kPlanPer];
     int sq = 0, sn = 0;
     unsigned int bad = 0, okm = 0;
-    const int head = max(0, *d.free_head), avail = max(0, d.n_free - head);
+    const int head0 = *d.free_head, head = max(0, head0), avail = max(0, d.n_free - head);
+    if (head0 < 0 || head0 > d.n_free) bad |= WASTE_CUDA_DERR_BAD_BLOCK;
 #pragma unroll
     for (int k = 0; k < kPlanPer; k++) {
         q[k] = need[k] = held[k] = 0;
@@ -108,7 +109,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(
         const int r = r0 + k;
         if (k >= per || r >= d.B) continue;
         const bool served = ((okm >> k) & 1) && (need[k] == 0 || pn + need[k] <= avail);
-        s.fstart[r] = served ? head + pn : -1;
+        s.fstart[r] = !served ? -1 : need[k] ? head + pn : 0;        /* 0: takes none, any place */
         if (served && need[k]) given = max(given, pn + need[k]);
         s.held[r] = held[k];
         pn = min(pn + need[k], 0x3fffffff);
