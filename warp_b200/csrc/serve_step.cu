@@ -679,14 +679,14 @@ cudaError_t logits_launch(const waste_cuda_logits_desc *d, unsigned int *err, in
 
 extern "C" {
 
-int wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, void *stream)
+int wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, int sms, void *stream)
 {
     const size_t smem = sizeof(PlanSmem);
     cudaError_t e = cudaFuncSetAttribute(kv_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          (int)smem);
     if (e != cudaSuccess) return (int)e;
     /* a token a thread. Counts updated in place need the cluster's barrier, so
-     * a portable cluster's size; else any number of CTAs */
+     * a portable cluster's size; else any number of CTAs, one an SM at most */
     const bool inplace = d->n_blocks == d->n_blocks_out || d->free_head == d->free_head_out;
     int n = (d->T + kPlanThreads - 1) / kPlanThreads;
     n = n < 1 ? 1 : n;
@@ -694,8 +694,8 @@ int wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, void 
         int c = 1;
         while (c < 8 && c < n) c <<= 1;
         n = c;
-    } else if (n > 148) {
-        n = 148;
+    } else if (n > sms) {
+        n = sms;
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n);

@@ -3365,7 +3365,7 @@ int waste_cuda_kv_plan_dev(const waste_cuda_kv_plan_desc *d, void *stream)
     if (misaligned(d->slot, 8)) return fail(WASTE_CUDA_E_ARG, "kv_plan_dev: slot is not 8-byte aligned");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("kv_plan_dev"))) goto out;
-    CK((cudaError_t)wc_kv_plan_launch(d, S.d_serr, stream ? stream : (void *)S.stream), "kv_plan");
+    CK((cudaError_t)wc_kv_plan_launch(d, S.d_serr, S.sms, stream ? stream : (void *)S.stream), "kv_plan");
 out:
     pthread_mutex_unlock(&g_mu);
     return rc;

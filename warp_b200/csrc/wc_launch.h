@@ -361,7 +361,7 @@ int wc_mla_gate_launch(float *o, const float *g, int n, void *stream, int pdl);
  * the descriptors are the public ones of waste_cuda.h, checked by the
  * caller. err: the sticky error word. sms: the device's SM count, which
  * sizes the attention's grid and workspace. */
-int    wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, void *stream);
+int    wc_kv_plan_launch(const waste_cuda_kv_plan_desc *d, unsigned int *err, int sms, void *stream);
 int    wc_mla_rows_launch(const waste_cuda_mla_rows_desc *d, unsigned int *err, void *stream);
 size_t wc_mla_tree_ws_bytes(int kl, int sms);
 int    wc_mla_tree_box(const waste_cuda_mla_tree_desc *d);
