@@ -762,8 +762,8 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * (else BAD_TREE: the request's new rows past that are seen by none).
  * q_indptr does not decrease and lies in 0..T (else BAD_BLOCK, and the call
  * writes nothing).
- * n_blocks: blocks in the cache. o overlaps no input. ws: waste_cuda_mla_tree_ws_bytes(heads,
- * kl) bytes on the device, 256-byte aligned, not shared by calls that may
+ * n_blocks: blocks in the cache. o overlaps no input, and its rows not each
+ * other. ws: waste_cuda_mla_tree_ws_bytes(heads, kl) bytes on the device, 256-byte aligned, not shared by calls that may
  * overlap (another stream, another captured graph); nothing in it has to
  * be set, or survives the call. Results do not depend on what runs beside
  * the call: sums are in a fixed order. */

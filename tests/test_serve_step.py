@@ -83,6 +83,9 @@ REFUSED = [
     ("kv_plan_dev", plan, dict(pos=A, slot=A)), ("kv_plan_dev", plan, dict(n_blocks_out=A, kv_len=A)),
     ("kv_plan_dev", plan, dict(mask_words=1 << 26)), ("mla_tree_attn_dev", tree, dict(mask_words=1 << 26)),
     ("logits_adjust_dev", logits, dict(tree_words=1 << 26)),
+    ("mla_tree_attn_dev", tree, dict(o_token_stride=512)), ("mla_tree_attn_dev", tree, dict(o_token_stride=1024)),
+    ("mla_tree_attn_dev", tree, dict(o_token_stride=512 * 31 + 511)), ("mla_tree_attn_dev", tree, dict(o_token_stride=700, o_head_stride=1000)),
+    ("mla_tree_attn_dev", tree, dict(o_token_stride=512, o_head_stride=512 * 4 - 1)),
 ]
 
 
@@ -92,6 +95,20 @@ def test_refused(lib, name, make, wrong):
     with pytest.raises(wb.WasteCudaError) as e:
         getattr(wb, name)(make(**wrong))
     assert e.value.rc == wb.E_ARG and name in str(e.value)
+
+
+@pytest.mark.parametrize("ts,hs,T,heads", [(512 * 32, 512, 4, 32), (512, 512 * 4, 4, 32), (512 * 31 + 512, 512, 4, 32),
+                                           (520, 4 * 520 - 8, 4, 32), (1024, 1024 * 4 + 512, 4, 32), (512, 512, 1, 32),
+                                           (512, 512, 4, 1), (1024, 1536, 2, 2), (1 << 62, 1 << 57, 4, 32)])
+def test_attn_rows_apart(lib, ts, hs, T, heads):
+    """Layouts of o whose rows share nothing pass the checks (and ask for a device)."""
+    if wb.load_library().waste_cuda_device() >= 0:
+        pytest.skip("another test bound the library")
+    with pytest.raises(wb.WasteCudaError) as e:
+        wb.mla_tree_attn_dev(tree(o_token_stride=ts, o_head_stride=hs, T=T, heads=heads))
+    taken = sorted(t * ts + h * hs for t in range(T) for h in range(heads))
+    assert all(b - a >= 512 for a, b in zip(taken, taken[1:]))
+    assert e.value.rc == wb.E_NODEV
 
 
 def test_null_descriptors(lib):

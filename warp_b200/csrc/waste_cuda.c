@@ -3321,6 +3321,19 @@ static int overlap(const void *a, size_t n, const void *b, size_t m)
     return n && m && (uintptr_t)a < (uintptr_t)b + m && (uintptr_t)b < (uintptr_t)a + n;
 }
 
+/* Two of T x H rows of n elements, ts and hs apart, share some */
+static int rows_overlap(int T, int H, size_t ts, size_t hs, size_t n)
+{
+    typedef unsigned __int128 u128;
+    if (T < 2 || H < 2) return (T > 1 && ts < n) || (H > 1 && hs < n);
+    if (ts >= (u128)(H - 1) * hs + n || hs >= (u128)(T - 1) * ts + n) return 0;
+    for (int h = 1; h < H; h++) {                /* neither lies within the other's step */
+        const u128 at = (u128)h * hs, t = at / ts, off = at % ts;
+        if ((t < (unsigned)T && off < n) || (t + 1 < (unsigned)T && ts - off < n)) return 1;
+    }
+    return 0;
+}
+
 /* The caller holds g_mu: the library is bound and its device is current. */
 static int serve_ready(const char *what)
 {
@@ -3417,6 +3430,8 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
         (d->mask && !words_ok(d->mask_words)) || misaligned(d->q, z) || misaligned(d->cache, z) ||
         misaligned(d->o, z) || misaligned(d->ws, 256) || d->o == d->q || d->o == d->cache)
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
+    if (rows_overlap(d->T, d->heads, d->o_token_stride, d->o_head_stride, (size_t)d->kl))
+        return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: rows of o overlap");
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("mla_tree_attn_dev"))) goto out;
     /* the kernels count (32 rows, 32 keys) units in 32 bits */
