@@ -766,7 +766,12 @@ int waste_cuda_mla_rows_dev(const waste_cuda_mla_rows_desc *d, void *stream);
  * other. ws: waste_cuda_mla_tree_ws_bytes(heads, kl) bytes on the device, 256-byte aligned, not shared by calls that may
  * overlap (another stream, another captured graph); nothing in it has to
  * be set, or survives the call. Results do not depend on what runs beside
- * the call: sums are in a fixed order. */
+ * the call: sums are in a fixed order.
+ * Limits, of the sizes that the host knows (not of the lengths): T * heads up
+ * to 2^25, and (T * heads / 32 + B + 1) * (page * max_blocks / 32 + 2) below
+ * 2^31 (a table as wide as the requests can get, no wider). The sums behind
+ * o are divided at the end, of weights up to 2^6 (2^14 in fp16): what the rows
+ * hold times that and their number has to stay within 32 bits' range. */
 typedef struct {
     int B, T, heads, kl, rope, dtype, page, max_blocks, mask_words;
     int64_t n_blocks;

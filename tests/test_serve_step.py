@@ -86,6 +86,8 @@ REFUSED = [
     ("mla_tree_attn_dev", tree, dict(o_token_stride=512)), ("mla_tree_attn_dev", tree, dict(o_token_stride=1024)),
     ("mla_tree_attn_dev", tree, dict(o_token_stride=512 * 31 + 511)), ("mla_tree_attn_dev", tree, dict(o_token_stride=700, o_head_stride=1000)),
     ("mla_tree_attn_dev", tree, dict(o_token_stride=512, o_head_stride=512 * 4 - 1)),
+    ("mla_tree_attn_dev", tree, dict(T=(1 << 20) + 1)), ("mla_tree_attn_dev", tree, dict(T=1 << 19, max_blocks=1 << 13)),
+    ("mla_tree_attn_dev", tree, dict(B=1 << 28, max_blocks=1 << 9)),
 ]
 
 
@@ -109,6 +111,22 @@ def test_attn_rows_apart(lib, ts, hs, T, heads):
     taken = sorted(t * ts + h * hs for t in range(T) for h in range(heads))
     assert all(b - a >= 512 for a, b in zip(taken, taken[1:]))
     assert e.value.rc == wb.E_NODEV
+
+
+def test_attn_limits(lib):
+    """The largest sizes the header allows pass the checks, one more is refused
+    with the numbers."""
+    if wb.load_library().waste_cuda_device() >= 0:
+        pytest.skip("another test bound the library")
+    units = lambda T, heads, B, cols, page: (T * heads // 32 + B + 1) * (page * cols // 32 + 2)
+    cols = next(c for c in range(1, 1 << 20) if units(64, 32, 2, c + 1, 1 << 11) >= 1 << 31)
+    for kw in (dict(T=1 << 20), dict(T=64, max_blocks=cols, page=1 << 11)):
+        with pytest.raises(wb.WasteCudaError) as e:
+            wb.mla_tree_attn_dev(tree(**kw))
+        assert e.value.rc == wb.E_NODEV, kw
+    with pytest.raises(wb.WasteCudaError) as e:
+        wb.mla_tree_attn_dev(tree(T=64, max_blocks=cols + 1, page=1 << 11))
+    assert e.value.rc == wb.E_ARG and str(units(64, 32, 2, cols + 1, 1 << 11)) in str(e.value)
 
 
 def test_null_descriptors(lib):

@@ -3432,15 +3432,15 @@ int waste_cuda_mla_tree_attn_dev(const waste_cuda_mla_tree_desc *d, void *stream
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: a missing or misaligned array");
     if (rows_overlap(d->T, d->heads, d->o_token_stride, d->o_head_stride, (size_t)d->kl))
         return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: rows of o overlap");
+    /* the kernels count (32 rows, 32 keys) units in 32 bits */
+    const int64_t rows = (int64_t)d->T * d->heads;
+    const int64_t units = (rows / 32 + d->B + 1) * ((int64_t)d->page * d->max_blocks / 32 + 2);
+    if (rows > 1 << 25 || units > INT32_MAX)
+        return fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: %d tokens of %d heads (2^25 rows at most) over tables of "
+                    "%d blocks of %d: %lld units of 32 x 32, 2^31 - 1 at most", d->T, d->heads, d->max_blocks, d->page,
+                    (long long)units);
     pthread_mutex_lock(&g_mu);
     if ((rc = serve_ready("mla_tree_attn_dev"))) goto out;
-    /* the kernels count (32 rows, 32 keys) units in 32 bits */
-    if ((int64_t)d->T * d->heads > 1 << 25 ||
-        ((int64_t)d->T * d->heads / 32 + d->B + 1) * ((int64_t)d->page * d->max_blocks / 32 + 2) > INT32_MAX) {
-        rc = fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: %d tokens of %d heads over %d blocks of %d", d->T,
-                  d->heads, d->max_blocks, d->page);
-        goto out;
-    }
     if (d->ws_bytes < wc_mla_tree_ws_bytes(d->kl, S.sms)) {
         rc = fail(WASTE_CUDA_E_ARG, "mla_tree_attn_dev: workspace of %zu bytes, %zu needed", d->ws_bytes,
                   wc_mla_tree_ws_bytes(d->kl, S.sms));
