@@ -31,9 +31,6 @@ using namespace wc;
 
 namespace {
 
-constexpr int kMaxKl = 512;
-constexpr int kMaxRope = 128;
-
 template <typename T> __device__ __forceinline__ float to_f(T v);
 template <> __device__ __forceinline__ float to_f(float v) { return v; }
 template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
@@ -496,7 +493,9 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  * of the call's rows a request, which the host knows: 64 tokens of 32 heads in
  * 64 requests take 61 us at N = 32 and 74 at 64; trees of up to 16 nodes 133
  * and 109; 2 trees of up to 5 over 131003 rows 224 and 183; 512 tokens over
- * 8192 rows 657 and 433.
+ * 8192 rows 657 and 433. In one call (L2 flushed before each) 512 tokens behind
+ * 4096 rows beside 63 single ones take 488 and 361, 64 beside them 125 and 125.
+ * Rows of T behind the last request's count towards the mean.
  *
  * Shared memory (1 CTA an SM): a ring of 32 KB pairs (128 keys x 2 swizzled
  * 64-column chunks) that TMA fills page by page, 5 pairs at N = 32 and 4 at
@@ -514,16 +513,20 @@ __global__ void __launch_bounds__(kGenThreads, 1) mla_gen_kernel(const __grid_co
  * times after, are the tile's maxima found (redux over the lanes, shared
  * memory over the 4 warps), the reference moved and O in TMEM rescaled.
  *
- * What bounds it. N = 32: 64 tokens over 183 k bf16 rows (216 MB) take 60 us
- * with the joining (60 to 61 from run to run), 3.5 TB/s. Traced tiles took 6.7 to 7.5 k cycles, where
+ * What bounds it. N = 32: 64 tokens over 183 k bf16 rows (216 MB) take 61 us
+ * with the joining, 3.5 TB/s. Traced tiles took 6.7 to 7.5 k cycles, where
  * 147 KB at an SM's share of HBM would take 6.4 k. At some ten tiles a CTA that
  * accounts for 36 us or so; the start (lengths, table, first tile: loads that
  * wait for one another), the end and the joining are left with the rest. N =
  * 64, the chain of a tile in one SM's shared memory: a tile is loaded (from L2:
  * 2.5 k cycles at 64 rows a box, 3.4 k at 32), its scores (36 products of 48
  * cycles, under the loads), the softmax 1.5 k, the second product 1.6 k. 512
- * tokens of 32 heads over 8192 rows take 433 us, 696 TFLOP/s; trees of up to 16
- * nodes for 16 requests 109 us. Measured and slower: V loaded again instead of held,
+ * tokens of 32 heads over 8192 rows take 434 us, 695 TFLOP/s, at 115 tiles a CTA
+ * 7.4 k cycles each, so there the chain is all. Trees of up to 16 nodes for 16
+ * requests take 109 us at 16.6 tiles a CTA, 12.9 k each: half of it is the start
+ * and end of query tiles and the joining. Two trees over 131003 rows take 183 us,
+ * 12.2 k a tile: a request's query tiles sweep its rows out of step, which reads
+ * 481 MB from HBM for 246 MB of rows. Measured and slower: V loaded again instead of held,
  * for an N of 96 (554 us where N = 64 took 445), rows sent for towards L2 two
  * tiles ahead (64 tokens: 62 -> 70 us).
  *
@@ -957,7 +960,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                 const int at = g.row0 + st, tok = at / H, h = at - tok * H;
                 const bool in = st < g.rows;
                 c.tok[st] = in ? tok : 0x3fffffff;
-                c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * d.q_head_stride : -1;
+                c.qoff[st] = in ? (long long)(g.q.q0 + tok) * (long long)d.q_token_stride + (long long)h * (long long)d.q_head_stride : -1ll;
                 c.ooff[o][st] = (long long)(g.q.q0 + tok) * (long long)d.o_token_stride + (long long)h * d.o_head_stride;
             }
         };
@@ -1128,6 +1131,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) mla_tc_kernel(const __grid_cons
                     }
                     __syncwarp();
                 }
+                /* the weights in the type of the rows, as the products take both operands
+                 * in one type: each is off by half a step at most (2^-8 in bf16, 2^-11 in
+                 * fp16), independent errors that leave o of 64 tokens in bf16 2.0e-3
+                 * from 64 bits where weights of 32 bits leave 1.7e-3, its own rounding.
+                 * Weights in two parts would double the product. The sums are of the
+                 * unrounded ones. */
                 uint32_t pk[NC / 2];
 #pragma unroll
                 for (int i = 0; i < NC; i += 2) {

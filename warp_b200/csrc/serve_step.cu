@@ -38,10 +38,10 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __
  * keeps them in shared memory, and takes its share of the tokens and table
  * entries. Where the counts are updated in place the CTAs are one cluster (at
  * most 8): its barrier stands between the last read of an input and the first
- * write. 64 requests of one token take 7.3 to 7.6 us a call from run to run
- * (launch included), 256 trees of up to 31 nodes 8.2. Which slot a token gets follows from
- * the old table (blocks held) or the free list (blocks taken now), so no
- * table entry written here is read here. */
+ * write. 64 requests of one token take 4.2 us in a captured graph, 256 trees of
+ * up to 31 nodes 6.4 (7.5 and 8.2 called one by one, which is the host's rate).
+ * Which slot a token gets follows from the old table (blocks held) or the free
+ * list (blocks taken now), so no table entry written here is read here. */
 constexpr int kPlanThreads = 512;
 constexpr int kPlanMaxB = 4096;
 constexpr int kPlanPer = kPlanMaxB / kPlanThreads;
@@ -218,7 +218,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv_plan_kernel(
  * again), so x crosses memory once: the bytes bound it at prompt lengths, a
  * launch and one row's latency at decode. Everything a row needs is loaded
  * before anything waits; where rows allow it four values a load (VEC 4), which
- * took 8191 rows of 512 + 64 floats to fp16 from 12.5 to 7.3 us (7.3 to 7.7 from run to run). */
+ * took 8191 rows of 512 + 64 floats to fp16 from 12.5 us a call to 7.4, the
+ * host's rate; in a captured graph they take 4.5, 64 rows 1.8. */
 constexpr int kRowsWarps = 4;
 constexpr int kRowRegs = 16;         /* 512 latents */
 
@@ -325,8 +326,8 @@ __global__ void __launch_bounds__(kRowsWarps * 32) mla_rows_kernel(
  * named values: with 8192, which two CTAs an SM still have room for, the cases
  * below took 21 us, and 103 on either side of 4096 named ids.
  * 64 rows of 163840 16-bit logits take 18 us (43 MB: 6.6 us of copying), 187
- * fp32 rows of 16 trees 76 to 78 us (247 MB: 38 us) where no slice names more
- * than kLogCap ids, and 102 to 105 where one does (165 with pieces of always
+ * fp32 rows of 16 trees 75 to 78 us (247 MB: 38 us) where no slice names more
+ * than kLogCap ids, and 100 to 105 where one does (165 with pieces of always
  * kLogCap ids). Measured and slower: counts for every id, in several waves (33 us), the rows staged in shared memory (67),
  * the sparse half following the copy row by row (20 and 85), the sparse work
  * as a kernel of its own under the copy (24 and 94).
